@@ -282,6 +282,34 @@ def decode_split_plan(batch: int, kv_heads: int, max_blocks: int, num_sms: int =
     return splits, bps
 
 
+def attn_tree(q, k_cache, v_cache, block_tables, seq_lens, row_start, out, layer: int,
+              scale: float, masks=None, k_scale=None, v_scale=None, max_nodes: int = 64,
+              workspace: Optional[GemmWorkspace] = None):
+    """Attention of the newest tokens of every sequence over the paged bf16
+    cache or, with ``k_scale`` / ``v_scale``, the 8-bit one: a single token
+    (plain decoding), a chain or a tree of drafted tokens.
+
+    q, out [rows, Hq * D] bf16; sequence b has the rows ``row_start[b] ..
+    row_start[b + 1]`` (int32 [B + 1]), whose K / V are the last keys of the
+    ``seq_lens[b]`` that its block table holds.  Row i of a sequence sees all
+    keys before its rows' own and, of those, key j iff bit j of its ``masks``
+    entry (int64 [rows]) is set; without masks the keys j <= i.  A row that
+    sees nothing gives zeros.  Lengths are read on the device, so a captured
+    graph follows them.  ``max_nodes``: an upper bound on the rows of a
+    sequence (at most 64 with masks)."""
+    if _dbg.ENABLED and not torch.cuda.is_current_stream_capturing():
+        _dbg.check_paged(block_tables, seq_lens, k_cache.shape[1])
+        _dbg.check_range("rows", row_start[1:] - row_start[:-1], 0, max_nodes + 1)
+    e = ext()
+    ws = workspace or default_workspace(q.device)
+    plan = e.attn_tree_plan(k_cache.shape[4])
+    ws.ensure(plan[1], plan[2])
+    e.attn_tree(q, k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, row_start, masks,
+                out, layer, scale, max_nodes, ws.ws, ws.counters)
+    LAUNCHES.add(1)
+    return out
+
+
 def prefill_tiles(q_lens, ctx_lens, device) -> torch.Tensor:
     """Per 64-row query tile: (seq, first packed row, first position, rows)."""
     tiles = []
@@ -329,6 +357,64 @@ def rope_kv_write(qkv, positions, cos_sin, slots, k_cache, v_cache, layer, hq, h
     ext().rope_kv_write(qkv, positions, cos_sin, slots, k_cache, v_cache, layer, hq, hkv, d, rot,
                         interleaved)
     LAUNCHES.add(1)
+
+
+def rope_kv_write_fp8(qkv, positions, cos_sin, slots, k_cache, v_cache, k_scale, v_scale,
+                      layer: int, hq: int, hkv: int, d: int, rot: int, interleaved: bool = False,
+                      q_out=None):
+    """RoPE of the q and k heads of a fused qkv row, K and V quantised into
+    the 8-bit paged cache: e4m3 codes [L, NB, Hkv, 16, D] and one fp32 scale
+    per (token, kv head), [L, NB, Hkv, 16].  The rotated q heads go to
+    ``q_out`` ([T, >= Hq * D] bf16) or, without it, back into ``qkv``.  Rows
+    whose slot is negative write no K / V."""
+    if _dbg.ENABLED and not torch.cuda.is_current_stream_capturing():
+        _dbg.check_range("kv slots", slots, 0, k_cache.shape[1] * 16, allow=(-1,))
+        _dbg.check_range("positions", positions, 0, cos_sin.shape[0])
+    ext().rope_kv_write_fp8(qkv, positions, cos_sin, slots, k_cache, v_cache, k_scale, v_scale,
+                            layer, hq, hkv, d, rot, interleaved, q_out)
+    LAUNCHES.add(1)
+
+
+def kv_read_fp8(k_cache, v_cache, k_scale, v_scale, blocks, layer: int, k_out=None, v_out=None):
+    """Blocks of the 8-bit cache back as bf16: two [N, Hkv, 16, D] tensors
+    (``k_out`` / ``v_out`` when given) for the N entries of ``blocks``
+    (int32; a negative entry gives zeros)."""
+    if _dbg.ENABLED and not torch.cuda.is_current_stream_capturing():
+        _dbg.check_range("blocks", blocks.clamp_min(-1), 0, k_cache.shape[1], allow=(-1,))
+    shape = (blocks.numel(),) + tuple(k_cache.shape[2:])
+    if k_out is None:
+        k_out = torch.empty(shape, dtype=torch.bfloat16, device=k_cache.device)
+    if v_out is None:
+        v_out = torch.empty(shape, dtype=torch.bfloat16, device=k_cache.device)
+    ext().kv_read_fp8(k_cache, v_cache, k_scale, v_scale, blocks, layer, k_out, v_out)
+    LAUNCHES.add(1)
+    return k_out, v_out
+
+
+def token_logprobs(logits, tokens, top_k: int = 0, workspace: Optional[GemmWorkspace] = None):
+    """Log-probabilities under softmax(logits): for every row of ``logits``
+    ([R, V] bf16, fp16 or fp32, any row stride) the log-probability of its
+    entry of ``tokens`` (int32 [R]), the entropy of the row in nats, and the
+    ``top_k`` (at most 32) most likely tokens with their log-probabilities,
+    ties to the lower id.  Returns (logprob [R], entropy [R], ids int32
+    [R, k], top [R, k]), fp32.
+
+    A row of nothing but -inf gives log-probabilities -inf and entropy 0; a
+    NaN or +inf in the row gives NaN (a NaN ranks before every number), and so
+    does a token outside the vocabulary."""
+    R, V = logits.shape
+    e = ext()
+    dev = logits.device
+    plan = e.token_logprobs_plan(R, V, logits.element_size())
+    ws = workspace or default_workspace(dev)
+    ws.ensure(plan[1], plan[2])
+    lp = torch.empty(R, dtype=torch.float32, device=dev)
+    ent = torch.empty(R, dtype=torch.float32, device=dev)
+    ids = torch.empty(R, top_k, dtype=torch.int32, device=dev)
+    top = torch.empty(R, top_k, dtype=torch.float32, device=dev)
+    e.token_logprobs(logits, tokens, top_k, lp, ent, ids, top, ws.ws, ws.counters)
+    LAUNCHES.add(1)
+    return lp, ent, ids, top
 
 
 def argmax(logits, out_idx, out_val=None, idx_offset: int = 0):

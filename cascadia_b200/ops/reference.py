@@ -84,6 +84,83 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_pos: torch.Te
     return torch.einsum("hqk,khd->qhd", p, vf)
 
 
+# ----------------------------------------------------------------- 8-bit cache
+
+E4M3_MAX = 448.0
+KV_SCALE_MIN = 2.0 ** -100
+
+
+def quantise_rows(y: torch.Tensor):
+    """e4m3 codes and fp32 scales of rows [..., D]: s = max(max |y| / 448,
+    2^-100), code = e4m3(y / s) (nearest even, saturating).  A row with a NaN
+    or an infinity gets s = NaN and zero codes."""
+    y = y.float()
+    peak = y.abs().amax(-1)
+    fine = torch.isfinite(peak)
+    s = torch.where(fine, (peak * (1.0 / E4M3_MAX)).clamp_min(KV_SCALE_MIN),
+                    torch.full_like(peak, float("nan")))
+    c = (y * (1.0 / s).unsqueeze(-1)).clamp(-E4M3_MAX, E4M3_MAX)
+    c = torch.where(fine.unsqueeze(-1), c, torch.zeros_like(c))
+    return c.to(torch.float8_e4m3fn), s
+
+
+def dequantise_rows(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
+    return codes.float() * scales.unsqueeze(-1)
+
+
+def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float,
+                   masks: Optional[Sequence[int]] = None) -> torch.Tensor:
+    """Attention of one sequence's newest tokens: q [n, Hq, D], k / v
+    [len, Hkv, D] whose last n rows are the nodes' own.  Row i sees every key
+    before them and node j iff bit j of masks[i] (no masks: j <= i); a row
+    that sees nothing gives zeros."""
+    n, hq, d = q.shape
+    tk, hkv, _ = k.shape
+    dt = torch.float64 if q.dtype == torch.float64 else torch.float32
+    ctx = tk - n
+    j = torch.arange(tk, device=q.device) - ctx  # node number of each key
+    if masks is None:
+        sees = j[None, :] <= torch.arange(n, device=q.device)[:, None]
+    else:
+        m = torch.as_tensor(masks, dtype=torch.int64, device=q.device)
+        sees = (j < 0)[None, :] | ((j < 64)[None, :] &
+                                   (m[:, None] >> j.clamp(0, 63)[None, :] & 1).bool())
+    g = hq // hkv
+    kf, vf = (x.to(dt).repeat_interleave(g, dim=1) for x in (k, v))
+    s = torch.einsum("qhd,khd->hqk", q.to(dt), kf) * scale
+    s = s.masked_fill(~sees[None], float("-inf"))
+    top = s.amax(-1, keepdim=True) if tk else s.new_zeros(hq, n, 1)
+    p = torch.exp(s - torch.where(top == float("-inf"), torch.zeros_like(top), top))
+    # A hidden key's value must not meet its weight of zero: it may be a NaN.
+    o = torch.zeros(n, hq, d, dtype=dt, device=q.device)
+    for i in range(n):
+        o[i] = torch.einsum("hk,khd->hd", p[:, i, sees[i]], vf[sees[i]])
+    total = p.sum(-1).t().unsqueeze(-1)
+    return torch.where(total == 0, torch.zeros_like(o), o / total)
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0):
+    """(logprob, entropy, ids, top) of logit rows; see ops.token_logprobs."""
+    x = logits if logits.dtype == torch.float64 else logits.float()
+    m = x.amax(-1, keepdim=True)
+    bad = ~(m < float("inf"))
+    empty = m == float("-inf")
+    sh = x - torch.where(empty, torch.zeros_like(m), m)
+    e = torch.exp(sh)
+    S = e.sum(-1, keepdim=True)
+    lp = torch.where(bad, torch.full_like(x, float("nan")),
+                     torch.where(empty, torch.full_like(x, float("-inf")), sh - S.log()))
+    ent = -torch.where(e > 0, e * lp, torch.zeros_like(x)).sum(-1) / S[:, 0]
+    ent = torch.where(bad[:, 0], torch.full_like(ent, float("nan")),
+                      torch.where(empty[:, 0], torch.zeros_like(ent), ent))
+    ids = torch.sort(x, dim=-1, descending=True, stable=True).indices[:, :top_k]
+    t = tokens.long()
+    known = (t >= 0) & (t < x.shape[1])
+    got = lp.gather(1, t.clamp(0, x.shape[1] - 1).unsqueeze(1))[:, 0]
+    got = torch.where(known, got, torch.full_like(got, float("nan")))
+    return got, ent, ids.to(torch.int32), lp.gather(1, ids)
+
+
 def argmax(logits: torch.Tensor) -> torch.Tensor:
     """Row argmax, lowest index on ties (the reference's strict `>` scan)."""
     return torch.argmax(logits.float(), dim=-1).to(torch.int32)

@@ -1,0 +1,654 @@
+// Attention of the newest tokens of every sequence over the paged KV cache:
+// one token (plain decoding), a chain, or a tree of drafted tokens.
+//
+// Sequence b has seq_lens[b] keys; the last n_b = row_start[b+1] - row_start[b]
+// of them are its query rows' own ("nodes", node i at key len - n + i).  Every
+// node sees all earlier keys (the context) and, among the nodes, those its
+// 64-bit mask names (no masks: itself and the nodes before it).
+//
+// Cache: [L, NB, Hkv, 16, D] bf16, or e4m3 codes with one fp32 scale for each
+// (token, kv head) of K and of V, [L, NB, Hkv, 16].  With scales
+//
+//   t_j = (q . kc_j) ks_j scale log2(e) + log2 vs_j,     M = max_j t_j
+//   w_j = 2^(t_j - M),   out = sum_j w_j vc_j / sum_j (w_j / vs_j)
+//
+// so that the weights of the value codes stay in [0, 1] whatever the scales
+// are, for one exponential a score.  e4m3 codes are exact in fp16; q is brought
+// into fp16's range by a power of two of its own for every row, and the weights
+// are held as 2^15 w in fp16 (11 bits).  With the bf16 cache the weights are
+// rounded to bf16, as its values are.  Sums and statistics are fp32.
+//
+// Work split: the keys of all (sequence, kv head, row tile) jobs form one line
+// of 16-token blocks that is cut into equal pieces, one for each CTA, so a
+// batch of uneven contexts keeps every SM busy to the end.  Lengths are read
+// on the device: a captured graph stays right when they change.  A job cut by
+// piece ends is joined by the last CTA that finishes a part of it, in the order
+// of the parts (the result does not depend on which CTA that is).
+#include <torch/extension.h>
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <cuda_fp8.h>
+
+#include "common.cuh"
+#include "host_utils.h"
+#include "mma_frag.cuh"
+
+namespace cb {
+namespace tree {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kNegBig = -1e30f;
+constexpr int kMaxBatch = 4096;
+
+struct Args {
+  const __nv_bfloat16* q;
+  int64_t q_stride;
+  const uint8_t* k;
+  const uint8_t* v;
+  const float* ks;
+  const float* vs;
+  const int* table;
+  int64_t table_stride;
+  int table_width;
+  const int* seq_lens;
+  const int* row_start;
+  const int64_t* masks;
+  __nv_bfloat16* out;
+  int64_t out_stride;
+  float* part;    // [grid][2][rows][D + 2]
+  int* counters;  // [grid], zero between launches
+  int64_t layer_blocks;
+  int B, Hkv, G;
+  float scale_log2;
+};
+
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                        uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t pair) {
+  const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)pair, __NV_E4M3);
+  return (uint32_t)r.x | ((uint32_t)r.y << 16);
+}
+
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// Streaming load: a cache row is read once by one SM.
+__device__ __forceinline__ uint4 ldg_stream16(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint2 ldg_stream8(const void* p) {
+  uint2 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];"
+               : "=r"(v.x), "=r"(v.y)
+               : "l"(p));
+  return v;
+}
+
+struct SeqShape {
+  int n, len, nb, tiles;
+};
+
+__device__ __forceinline__ SeqShape seq_shape(const Args& a, int b, int rows) {
+  SeqShape s;
+  s.n = max(0, a.row_start[b + 1] - a.row_start[b]);
+  s.len = min(max(0, a.seq_lens[b]), a.table_width * 16);
+  s.nb = max(1, (s.len + 15) >> 4);
+  s.tiles = (s.n * a.G + rows - 1) / rows;
+  return s;
+}
+
+// pre[b] = 16-token blocks of work before sequence b; pre[B] = all of it.
+__device__ __forceinline__ void scan_work(const Args& a, int rows, int64_t* pre, int64_t* warp_sum) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int64_t carry = 0;
+  if (tid == 0) pre[0] = 0;
+  for (int base = 0; base < a.B; base += 128) {
+    const int b = base + tid;
+    int64_t u = 0;
+    if (b < a.B) {
+      const SeqShape s = seq_shape(a, b, rows);
+      u = (int64_t)a.Hkv * s.tiles * s.nb;
+    }
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t x = __shfl_up_sync(0xffffffffu, u, o);
+      if (lane >= o) u += x;
+    }
+    if (lane == 31) warp_sum[warp] = u;
+    __syncthreads();
+    int64_t before = carry;
+    for (int w = 0; w < 4; ++w) {
+      if (w < warp) before += warp_sum[w];
+      carry += warp_sum[w];
+    }
+    if (b < a.B) pre[b + 1] = before + u;
+    __syncthreads();
+  }
+}
+
+// One warp's view of one 16-token block: K and V as loaded, and the scales.
+template <int D, bool FP8>
+struct Block {
+  static constexpr int KC = FP8 ? D / 64 : D / 32;  // 16-byte K chunks of a lane and token
+  static constexpr int VW = FP8 ? D / 32 : D / 16;  // V words of a lane and token
+  uint4 k[2][KC];
+  uint32_t v[4][VW];
+  float2 ks[2], vs[2];
+
+  // Tokens of lane (g, t4): K rows g and 8 + g; V rows 2 t4, 2 t4 + 1 and
+  // those plus 8.  A lane's K chunk c holds the head dims of its k-steps (any
+  // order of the summed dims will do, if q has the same), its V words the
+  // D / 8 dims from g D / 8 on.
+  __device__ __forceinline__ void load(const Args& a, const int* table, int h, int blk, int g,
+                                       int t4) {
+    const int64_t row = ((a.layer_blocks + table[blk]) * a.Hkv + h) * 16;
+    constexpr int RB = FP8 ? D : 2 * D;  // bytes of a row
+    const uint8_t* kp = a.k + row * RB;
+    const uint8_t* vp = a.v + row * RB;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int c = 0; c < KC; ++c) k[i][c] = ldg_stream16(kp + (8 * i + g) * RB + c * 64 + t4 * 16);
+    if constexpr (FP8) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        ks[i] = *reinterpret_cast<const float2*>(a.ks + row + 8 * i + 2 * t4);
+        vs[i] = *reinterpret_cast<const float2*>(a.vs + row + 8 * i + 2 * t4);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint8_t* p = vp + (8 * (i >> 1) + 2 * t4 + (i & 1)) * RB + g * (RB / 8);
+      if constexpr (VW == 2) {
+        const uint2 u = ldg_stream8(p);
+        v[i][0] = u.x;
+        v[i][1] = u.y;
+      } else {
+#pragma unroll
+        for (int w = 0; w < VW / 4; ++w) {
+          const uint4 u = ldg_stream16(p + 16 * w);
+          v[i][4 * w] = u.x;
+          v[i][4 * w + 1] = u.y;
+          v[i][4 * w + 2] = u.z;
+          v[i][4 * w + 3] = u.w;
+        }
+      }
+    }
+  }
+};
+
+// 4 warps; each takes every fourth block of a job's keys for all 16 rows of the
+// job's tile and streams K and V from global memory straight into the operand
+// registers of its warp-level products (a row of 128 B is one whole line, and
+// no byte is used by two warps, so shared memory would only add a copy).
+template <int D, bool FP8>
+__global__ void __launch_bounds__(128) attn_rows_kernel(const Args a) {
+  constexpr int ROWS = 16;
+  constexpr int NKS = D / 16;
+  constexpr int NT = D / 8;
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  int64_t* pre = reinterpret_cast<int64_t*>(smem_raw);
+  float* sm_o = reinterpret_cast<float*>(smem_raw + ((a.B + 2) / 2 * 2) * 8);  // [4][16][D]
+  float* sm_ml = sm_o + 4 * ROWS * D;                                         // [4][16][2]
+  __shared__ int64_t s_sum[4];
+  __shared__ int s_last;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int g = lane >> 2, t4 = lane & 3;
+  grid_dep_launch();
+  grid_dep_wait();
+
+  scan_work(a, ROWS, pre, s_sum);
+  const int64_t total = pre[a.B];
+  // At least 8 blocks a piece: two for each warp.
+  const int64_t piece = max((int64_t)8, (total + gridDim.x - 1) / gridDim.x);
+  int64_t u = (int64_t)blockIdx.x * piece;
+  const int64_t u_end = min(total, u + piece);
+
+  while (u < u_end) {
+    int lo = 0, hi = a.B;  // pre[lo] <= u < pre[hi]
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (pre[mid] <= u) lo = mid;
+      else hi = mid;
+    }
+    // Sequences without rows share their successor's offset: the search ends
+    // on the last of them, the one with the work.
+    const int b = lo;
+    const SeqShape s = seq_shape(a, b, ROWS);
+    const int64_t local = u - pre[b];
+    const int job = (int)(local / s.nb);
+    const int k0 = (int)(local - (int64_t)job * s.nb);
+    const int k1 = (int)min((int64_t)s.nb, k0 + (u_end - u));
+    const int h = job / s.tiles, tile = job - h * s.tiles;
+    const int ctx = s.len - s.n;
+    const int* table = a.table + (int64_t)b * a.table_stride;
+    const int q_row0 = a.row_start[b];
+    const int rows_left = s.n * a.G - tile * ROWS;
+
+    // The two rows of this lane (g and g + 8 of the tile).
+    int node[2];
+    uint64_t mask[2];
+    float row_scale[2];
+    uint32_t qa[NKS][4];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int rr = tile * ROWS + g + 8 * r;
+      const bool live = g + 8 * r < rows_left;
+      node[r] = live ? rr / a.G : 0;
+      const int head = h * a.G + (live ? rr - node[r] * a.G : 0);
+      mask[r] = 0;
+      if (live && a.masks != nullptr) mask[r] = (uint64_t)a.masks[q_row0 + node[r]];
+      const __nv_bfloat16* qp = a.q + (int64_t)(q_row0 + node[r]) * a.q_stride + (int64_t)head * D;
+      uint32_t top = 0;
+#pragma unroll
+      for (int ks = 0; ks < NKS; ++ks) {
+        const int d = FP8 ? (ks >> 2) * 64 + t4 * 16 + (ks & 3) * 4
+                          : (ks >> 1) * 32 + t4 * 8 + (ks & 1) * 4;
+        const uint2 w = live ? *reinterpret_cast<const uint2*>(qp + d) : make_uint2(0u, 0u);
+        qa[ks][r] = w.x;
+        qa[ks][2 + r] = w.y;
+        if constexpr (FP8) {
+          top = max(top, max(w.x & 0x7fffu, (w.x >> 16) & 0x7fffu));
+          top = max(top, max(w.y & 0x7fffu, (w.y >> 16) & 0x7fffu));
+        }
+      }
+      row_scale[r] = a.scale_log2;
+      if constexpr (FP8) {
+        // A power of two that puts the row's largest value into [2^14, 2^15):
+        // what it moves below fp16's smallest value is under 2^-38 of that.
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int e = (int)(top >> 7);  // biased exponent
+        const int sh = e == 0 || e == 255 ? 0 : min(100, 127 + 14 - e);
+        const float up = __int_as_float((127 + sh) << 23);
+        row_scale[r] *= __int_as_float((127 - sh) << 23);
+#pragma unroll
+        for (int ks = 0; ks < NKS; ++ks) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const uint32_t w = qa[ks][2 * k + r];
+            qa[ks][2 * k + r] = pack_f16(__uint_as_float(w << 16) * up,
+                                         __uint_as_float(w & 0xffff0000u) * up);
+          }
+        }
+      }
+    }
+
+    float o[NT][4];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    float m[2] = {kNegBig, kNegBig};
+    float l[2] = {0.f, 0.f};
+
+    const int blk_end = min(k1, (s.len + 15) >> 4);
+    Block<D, FP8> x;
+    for (int blk = k0 + warp; blk < blk_end; blk += 4) {
+      x.load(a, table, h, blk, g, t4);
+      const int pos0 = blk * 16;
+      float sc[2][4];
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt) {
+        sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
+#pragma unroll
+        for (int c = 0; c < Block<D, FP8>::KC; ++c) {
+          const uint32_t w[4] = {x.k[nt][c].x, x.k[nt][c].y, x.k[nt][c].z, x.k[nt][c].w};
+          if constexpr (FP8) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              mma_f16(sc[nt], qa[4 * c + i], e4m3x2_to_f16x2(w[i] & 0xffffu),
+                      e4m3x2_to_f16x2(w[i] >> 16));
+          } else {
+            mma_16816(sc[nt], qa[2 * c], w[0], w[1]);
+            mma_16816(sc[nt], qa[2 * c + 1], w[2], w[3]);
+          }
+        }
+      }
+      // Scores in base 2, hidden keys at -inf.
+      float inv_vs[2][2];
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt) {
+        float kk[2] = {1.f, 1.f}, lv[2] = {0.f, 0.f};
+        inv_vs[nt][0] = inv_vs[nt][1] = 1.f;
+        if constexpr (FP8) {
+          kk[0] = x.ks[nt].x;
+          kk[1] = x.ks[nt].y;
+          lv[0] = __log2f(x.vs[nt].x);
+          lv[1] = __log2f(x.vs[nt].y);
+          inv_vs[nt][0] = exp2f(-lv[0]);
+          inv_vs[nt][1] = exp2f(-lv[1]);
+        }
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            sc[nt][2 * r + e] = sc[nt][2 * r + e] * (kk[e] * row_scale[r]) + lv[e];
+      }
+      uint32_t hidden = 0;  // bit 4 nt + 2 r + e of this lane's scores
+      if (pos0 + 16 > ctx) {
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int pos = pos0 + 8 * nt + 2 * t4 + e;
+              const int j = pos - ctx;
+              bool sees = pos < s.len;
+              if (j >= 0)
+                sees = sees && (a.masks != nullptr ? j < 64 && ((mask[r] >> (j & 63)) & 1)
+                                                   : j <= node[r]);
+              if (!sees) {
+                sc[nt][2 * r + e] = -INFINITY;
+                hidden |= 1u << (4 * nt + 2 * r + e);
+              }
+            }
+        // Value rows past the end may hold anything: a weight of zero does
+        // not remove a NaN from a product.
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (pos0 + 8 * (i >> 1) + 2 * t4 + (i & 1) >= s.len) {
+#pragma unroll
+            for (int w = 0; w < Block<D, FP8>::VW; ++w) x.v[i][w] = 0u;
+          }
+      }
+      float p[2][4];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        float mx = fmaxf(fmaxf(sc[0][2 * r], sc[0][2 * r + 1]), fmaxf(sc[1][2 * r], sc[1][2 * r + 1]));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const float m_new = fmaxf(m[r], mx);
+        const float alpha = exp2f(m[r] - m_new);
+        const float base = FP8 ? m_new - 15.f : m_new;
+        float sum = 0.f;
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float w = exp2f(sc[nt][2 * r + e] - base);
+            // A NaN scale of a hidden key must not reach the sum either.
+            if (hidden >> (4 * nt + 2 * r + e) & 1) w = 0.f;
+            else sum += FP8 ? w * inv_vs[nt][e] : w;
+            p[nt][2 * r + e] = w;
+          }
+        l[r] = l[r] * alpha + sum;
+        m[r] = m_new;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          o[nt][2 * r] *= alpha;
+          o[nt][2 * r + 1] *= alpha;
+        }
+      }
+      uint32_t pa[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        pa[i] = FP8 ? pack_f16(p[i >> 1][2 * (i & 1)], p[i >> 1][2 * (i & 1) + 1])
+                    : pack_bf16(p[i >> 1][2 * (i & 1)], p[i >> 1][2 * (i & 1) + 1]);
+      if constexpr (!FP8) {
+        // A node may hold an infinity or a NaN that its siblings do not see:
+        // those values leave the product and are added to the rows that do.
+        if (pos0 + 16 > ctx) {
+          bool bad = false;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int w = 0; w < Block<D, FP8>::VW; ++w) {
+              uint32_t y = x.v[i][w];
+              if ((y & 0x7f80u) == 0x7f80u) { y &= 0xffff0000u; bad = true; }
+              if ((y & 0x7f800000u) == 0x7f800000u) { y &= 0xffffu; bad = true; }
+              x.v[i][w] = y;
+            }
+          if (__any_sync(0xffffffffu, bad)) {
+            const int64_t row = ((a.layer_blocks + table[blk]) * a.Hkv + h) * 16;
+            const __nv_bfloat16* vp = reinterpret_cast<const __nv_bfloat16*>(a.v) + row * D;
+            for (int tok = 0; tok < 16 && pos0 + tok < s.len; ++tok) {
+              const int j = pos0 + tok - ctx;
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  const float val = __bfloat162float(vp[tok * D + (2 * t4 + e) * NT + nt]);
+                  if (!(fabsf(val) <= 3.4e38f)) {
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                      const bool sees =
+                          j < 0 || (a.masks != nullptr ? j < 64 && ((mask[r] >> (j & 63)) & 1)
+                                                       : j <= node[r]);
+                      if (sees) o[nt][2 * r + e] += val;
+                    }
+                  }
+                }
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int w = 0; w < Block<D, FP8>::VW; ++w) {
+        if constexpr (FP8) {
+          // Bytes of the two tokens side by side, four dims a word.
+          const uint32_t a0 = __byte_perm(x.v[0][w], x.v[1][w], 0x5140);
+          const uint32_t a1 = __byte_perm(x.v[0][w], x.v[1][w], 0x7362);
+          const uint32_t b0 = __byte_perm(x.v[2][w], x.v[3][w], 0x5140);
+          const uint32_t b1 = __byte_perm(x.v[2][w], x.v[3][w], 0x7362);
+          mma_f16(o[4 * w], pa, e4m3x2_to_f16x2(a0 & 0xffffu), e4m3x2_to_f16x2(b0 & 0xffffu));
+          mma_f16(o[4 * w + 1], pa, e4m3x2_to_f16x2(a0 >> 16), e4m3x2_to_f16x2(b0 >> 16));
+          mma_f16(o[4 * w + 2], pa, e4m3x2_to_f16x2(a1 & 0xffffu), e4m3x2_to_f16x2(b1 & 0xffffu));
+          mma_f16(o[4 * w + 3], pa, e4m3x2_to_f16x2(a1 >> 16), e4m3x2_to_f16x2(b1 >> 16));
+        } else {
+          mma_16816(o[2 * w], pa, __byte_perm(x.v[0][w], x.v[1][w], 0x5410),
+                    __byte_perm(x.v[2][w], x.v[3][w], 0x5410));
+          mma_16816(o[2 * w + 1], pa, __byte_perm(x.v[0][w], x.v[1][w], 0x7632),
+                    __byte_perm(x.v[2][w], x.v[3][w], 0x7632));
+        }
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+    }
+
+    // Join the four warps, then the CTAs that share the job.
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int row = g + 8 * r;
+      if (row < rows_left) {
+        float* dst = sm_o + (warp * ROWS + row) * D;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          dst[2 * t4 * NT + nt] = o[nt][2 * r];
+          dst[(2 * t4 + 1) * NT + nt] = o[nt][2 * r + 1];
+        }
+        if (t4 == 0) {
+          sm_ml[(warp * ROWS + row) * 2] = m[r];
+          sm_ml[(warp * ROWS + row) * 2 + 1] = l[r];
+        }
+      }
+    }
+    __syncthreads();
+    const int64_t js = pre[b] + (int64_t)job * s.nb;
+    const int64_t c0 = js / piece, c1 = (js + s.nb - 1) / piece;
+    const int rows = min(ROWS, rows_left);
+    const bool whole = c0 == c1;
+    float* part = a.part + ((int64_t)blockIdx.x * 2 + (blockIdx.x == c0 ? 1 : 0)) * ROWS * (D + 2);
+    for (int idx = tid; idx < rows * D; idx += 128) {
+      const int row = idx / D, d = idx % D;
+      float M = kNegBig;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) M = fmaxf(M, sm_ml[(w * ROWS + row) * 2]);
+      float L = 0.f, O = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float f = exp2f(sm_ml[(w * ROWS + row) * 2] - M);
+        L += sm_ml[(w * ROWS + row) * 2 + 1] * f;
+        O += sm_o[(w * ROWS + row) * D + d] * f;
+      }
+      if (whole) {
+        const int rr = tile * ROWS + row;
+        a.out[(int64_t)(q_row0 + rr / a.G) * a.out_stride + (int64_t)(h * a.G + rr % a.G) * D + d] =
+            __float2bfloat16(L == 0.f ? 0.f : O / L);
+      } else {
+        part[row * (D + 2) + 2 + d] = O;
+        if (d == 0) {
+          part[row * (D + 2)] = M;
+          part[row * (D + 2) + 1] = L;
+        }
+      }
+    }
+    if (!whole) {
+      __threadfence();
+      __syncthreads();
+      if (tid == 0) {
+        const int parts = (int)(c1 - c0 + 1);
+        s_last = atomicAdd(a.counters + c0, 1) == parts - 1;
+        if (s_last) a.counters[c0] = 0;
+      }
+      __syncthreads();
+      if (s_last) {
+        __threadfence();
+        for (int idx = tid; idx < rows * D; idx += 128) {
+          const int row = idx / D, d = idx % D;
+          float M = kNegBig, L = 0.f, O = 0.f;
+          for (int64_t c = c0; c <= c1; ++c) {
+            const float* src =
+                a.part + (c * 2 + (c == c0 ? 1 : 0)) * ROWS * (D + 2) + row * (D + 2);
+            const float m_c = __ldcg(src), l_c = __ldcg(src + 1), o_c = __ldcg(src + 2 + d);
+            const float m_new = fmaxf(M, m_c);
+            const float f0 = exp2f(M - m_new), f1 = exp2f(m_c - m_new);
+            L = L * f0 + l_c * f1;
+            O = O * f0 + o_c * f1;
+            M = m_new;
+          }
+          const int rr = tile * ROWS + row;
+          a.out[(int64_t)(q_row0 + rr / a.G) * a.out_stride + (int64_t)(h * a.G + rr % a.G) * D +
+                d] = __float2bfloat16(L == 0.f ? 0.f : O / L);
+        }
+      }
+    }
+    __syncthreads();  // shared buffers are reused by the next job
+    u += k1 - k0;
+  }
+}
+
+template <int D, bool FP8>
+void launch_rows(const Args& a, int grid, cudaStream_t stream) {
+  const int smem = (a.B + 2) / 2 * 2 * 8 + 4 * 16 * (D + 2) * 4;
+  static int configured = 0;
+  if (smem > configured) {
+    CB_CUDA_CHECK(cudaFuncSetAttribute(attn_rows_kernel<D, FP8>,
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    configured = smem;
+  }
+  launch_kernel(attn_rows_kernel<D, FP8>, dim3(grid), dim3(128), smem, stream, a);
+}
+
+}  // namespace tree
+
+// {grid, workspace floats, workspace counters} of attn_tree.
+std::vector<int64_t> attn_tree_plan(int64_t head_dim) {
+  const int64_t grid = 2 * num_sms();
+  return {grid, grid * 2 * 16 * (head_dim + 2), grid};
+}
+
+// q, out: [rows, Hq * D]; rows of sequence b are row_start[b] .. row_start[b+1].
+void attn_tree(torch::Tensor q, torch::Tensor k_cache, torch::Tensor v_cache,
+               c10::optional<torch::Tensor> k_scale, c10::optional<torch::Tensor> v_scale,
+               torch::Tensor block_tables, torch::Tensor seq_lens, torch::Tensor row_start,
+               c10::optional<torch::Tensor> masks, torch::Tensor out, int64_t layer, double scale,
+               int64_t max_nodes, torch::Tensor ws, torch::Tensor counters) {
+  TORCH_CHECK(q.is_cuda() && q.dim() == 2 && q.scalar_type() == at::kBFloat16 &&
+                  out.dim() == 2 && out.scalar_type() == at::kBFloat16 && q.stride(1) == 1 &&
+                  out.stride(1) == 1 && out.size(0) >= q.size(0) && out.size(1) == q.size(1),
+              "q / out must be bf16 [rows, Hq * D] with inner stride 1");
+  TORCH_CHECK(k_cache.dim() == 5 && k_cache.size(3) == 16 && k_cache.is_contiguous() &&
+                  v_cache.is_contiguous() && v_cache.sizes() == k_cache.sizes() &&
+                  v_cache.scalar_type() == k_cache.scalar_type(),
+              "kv cache must be [L, NB, Hkv, 16, D] contiguous");
+  const bool fp8 = k_cache.scalar_type() == at::kFloat8_e4m3fn;
+  TORCH_CHECK(fp8 || k_cache.scalar_type() == at::kBFloat16,
+              "kv cache must be bf16 or float8_e4m3fn");
+  TORCH_CHECK(fp8 == k_scale.has_value() && fp8 == v_scale.has_value(),
+              "the 8-bit cache comes with k_scale and v_scale, the bf16 cache without");
+  const int D = (int)k_cache.size(4), Hkv = (int)k_cache.size(2);
+  TORCH_CHECK(D == 64 || D == 128, "head_dim must be 64 or 128");
+  TORCH_CHECK(q.size(1) % D == 0 && (q.size(1) / D) % Hkv == 0, "query heads must divide");
+  TORCH_CHECK(layer >= 0 && layer < k_cache.size(0), "layer outside the cache");
+  const int64_t B = seq_lens.numel();
+  TORCH_CHECK(B <= tree::kMaxBatch, "at most 4096 sequences");
+  TORCH_CHECK(block_tables.scalar_type() == at::kInt && block_tables.dim() == 2 &&
+                  block_tables.size(0) >= B && block_tables.stride(1) == 1 &&
+                  seq_lens.scalar_type() == at::kInt && seq_lens.is_contiguous() &&
+                  row_start.scalar_type() == at::kInt && row_start.is_contiguous() &&
+                  row_start.numel() >= B + 1,
+              "int32 block tables [B, W], seq lens [B] and row starts [B + 1]");
+  for (const torch::Tensor* t :
+       {&out, &k_cache, &v_cache, &block_tables, &seq_lens, &row_start, &ws, &counters})
+    TORCH_CHECK(t->device() == q.device(), "all tensors must be on one device");
+  if (fp8) {
+    for (const torch::Tensor* t : {&*k_scale, &*v_scale})
+      TORCH_CHECK(t->scalar_type() == at::kFloat && t->is_contiguous() &&
+                      t->numel() == k_cache.numel() / D && t->device() == q.device(),
+                  "k/v scales must be fp32 [L, NB, Hkv, 16] contiguous");
+  }
+  if (masks.has_value())
+    TORCH_CHECK(masks->scalar_type() == at::kLong && masks->is_contiguous() &&
+                    masks->numel() >= q.size(0) && masks->device() == q.device(),
+                "masks must be int64, one per row");
+  TORCH_CHECK(max_nodes >= 1 && (!masks.has_value() || max_nodes <= 64),
+              "a tree has at most 64 nodes");
+  TORCH_CHECK((q.stride(0) * 2) % 16 == 0 && reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0,
+              "q rows must be 16-byte aligned");
+  if (B == 0 || q.size(0) == 0) return;
+  const c10::cuda::CUDAGuard guard(q.device());
+  const std::vector<int64_t> plan = attn_tree_plan(D);
+  TORCH_CHECK(ws.scalar_type() == at::kFloat && ws.numel() >= plan[1] &&
+                  counters.scalar_type() == at::kInt && counters.numel() >= plan[2],
+              "workspace too small");
+  tree::Args a;
+  a.q = reinterpret_cast<const __nv_bfloat16*>(q.data_ptr());
+  a.q_stride = q.stride(0);
+  a.k = reinterpret_cast<const uint8_t*>(k_cache.data_ptr());
+  a.v = reinterpret_cast<const uint8_t*>(v_cache.data_ptr());
+  a.ks = fp8 ? k_scale->data_ptr<float>() : nullptr;
+  a.vs = fp8 ? v_scale->data_ptr<float>() : nullptr;
+  a.table = block_tables.data_ptr<int>();
+  a.table_stride = block_tables.stride(0);
+  a.table_width = (int)block_tables.size(1);
+  a.seq_lens = seq_lens.data_ptr<int>();
+  a.row_start = row_start.data_ptr<int>();
+  a.masks = masks.has_value() ? masks->data_ptr<int64_t>() : nullptr;
+  a.out = reinterpret_cast<__nv_bfloat16*>(out.data_ptr());
+  a.out_stride = out.stride(0);
+  a.part = ws.data_ptr<float>();
+  a.counters = counters.data_ptr<int>();
+  a.layer_blocks = layer * k_cache.size(1);
+  a.B = (int)B;
+  a.Hkv = Hkv;
+  a.G = (int)(q.size(1) / D / Hkv);
+  a.scale_log2 = (float)scale * tree::kLog2e;
+  cudaStream_t stream = at::cuda::getCurrentCUDAStream();
+  const int grid = (int)plan[0];
+  if (D == 128) {
+    if (fp8) tree::launch_rows<128, true>(a, grid, stream);
+    else tree::launch_rows<128, false>(a, grid, stream);
+  } else {
+    if (fp8) tree::launch_rows<64, true>(a, grid, stream);
+    else tree::launch_rows<64, false>(a, grid, stream);
+  }
+}
+
+}  // namespace cb

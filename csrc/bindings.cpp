@@ -114,6 +114,27 @@ void attn_decode(torch::Tensor q, torch::Tensor k_cache, torch::Tensor v_cache,
 void attn_prefill(torch::Tensor q, torch::Tensor k_cache, torch::Tensor v_cache,
                   torch::Tensor block_tables, torch::Tensor tiles, torch::Tensor out, int64_t layer,
                   double scale, torch::Tensor status, int64_t window, int64_t sinks);
+// kv_fp8.cu
+void rope_kv_write_fp8(torch::Tensor qkv, torch::Tensor positions, torch::Tensor cos_sin,
+                       torch::Tensor slots, torch::Tensor k_cache, torch::Tensor v_cache,
+                       torch::Tensor k_scale, torch::Tensor v_scale, int64_t layer, int64_t Hq,
+                       int64_t Hkv, int64_t D, int64_t rot, bool interleaved,
+                       c10::optional<torch::Tensor> q_out);
+void kv_read_fp8(torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor k_scale,
+                 torch::Tensor v_scale, torch::Tensor blocks, int64_t layer, torch::Tensor k_out,
+                 torch::Tensor v_out);
+// attn_tree.cu
+std::vector<int64_t> attn_tree_plan(int64_t head_dim);
+void attn_tree(torch::Tensor q, torch::Tensor k_cache, torch::Tensor v_cache,
+               c10::optional<torch::Tensor> k_scale, c10::optional<torch::Tensor> v_scale,
+               torch::Tensor block_tables, torch::Tensor seq_lens, torch::Tensor row_start,
+               c10::optional<torch::Tensor> masks, torch::Tensor out, int64_t layer, double scale,
+               int64_t max_nodes, torch::Tensor ws, torch::Tensor counters);
+// logprobs.cu
+std::vector<int64_t> token_logprobs_plan(int64_t rows, int64_t vocab, int64_t elem_size);
+void token_logprobs(torch::Tensor logits, torch::Tensor tokens, int64_t top_k,
+                    torch::Tensor logprob, torch::Tensor entropy, torch::Tensor top_ids,
+                    torch::Tensor top_lp, torch::Tensor ws, torch::Tensor counters);
 // elementwise.cu
 void embedding(torch::Tensor ids, torch::Tensor table, torch::Tensor out, int64_t vocab_lo);
 void rmsnorm(torch::Tensor x, c10::optional<torch::Tensor> residual, torch::Tensor w,
@@ -168,6 +189,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("attn_prefill", &cb::attn_prefill, py::arg("q"), py::arg("k_cache"), py::arg("v_cache"),
         py::arg("block_tables"), py::arg("tiles"), py::arg("out"), py::arg("layer"),
         py::arg("scale"), py::arg("status"), py::arg("window") = 0, py::arg("sinks") = 0);
+  m.def("rope_kv_write_fp8", &cb::rope_kv_write_fp8);
+  m.def("kv_read_fp8", &cb::kv_read_fp8);
+  m.def("attn_tree_plan", &cb::attn_tree_plan);
+  m.def("attn_tree", &cb::attn_tree);
+  m.def("token_logprobs_plan", &cb::token_logprobs_plan);
+  m.def("token_logprobs", &cb::token_logprobs);
   m.def("embedding", &cb::embedding);
   m.def("rmsnorm", &cb::rmsnorm);
   m.def("rope_kv_write", &cb::rope_kv_write);

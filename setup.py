@@ -32,6 +32,9 @@ SOURCES = [
     "mla.cu",
     "gdn.cu",
     "ffn_sparse.cu",
+    "kv_fp8.cu",
+    "attn_tree.cu",
+    "logprobs.cu",
 ]
 
 NVCC_FLAGS = [
