@@ -1,15 +1,24 @@
 // Log-probabilities of given tokens, entropy and the top alternatives of logit
 // rows, in one pass over the logits.
 //
-//   m = max x,  S = sum e^(x - m),  W = sum e^(x - m) (x - m)
-//   logprob(t) = (x_t - m) - ln S,   entropy = ln S - W / S
+//   S = sum 2^(x log2e - r),  W = sum 2^(x log2e - r) (x log2e - r)
+//   log2 p(t) = (x_t log2e - r) - log2 S,   entropy = ln 2 (log2 S - W / S)
 //
-// held as a running (m, S, W) by every thread and joined at the end.  The k-th
-// largest of the threads' largest values is a bound below the row's k-th
-// largest: only the at most k threads whose largest value reaches it can hold
-// any of the row's top k.  Order: larger value first, then lower index
-// (-0 = 0; a NaN comes before everything).  A row is cut in slices, one for each
-// CTA, when there are few rows; the last CTA of a row joins them.
+// hold for every reference r near the row's maximum: each thread keeps its own
+// (r, S, W) and moves r only when a value is 2^8 times over it, so the common
+// path is one fused multiply-add and one exponential a value (the same r stands
+// in every term, so its own rounding cancels).  Above 1e29 in magnitude two
+// different floats are so far apart that S is the number of values equal to
+// the maximum.
+//
+// Top k: each thread notes the chunk of its own largest value.  The k-th largest
+// of the threads' largest values is a bound below the row's k-th largest, and
+// only the at most k threads whose largest value reaches it can hold any of
+// the row's top k: their values alone are read a second time.  Order: larger
+// value first, then lower index (-0 = 0; a NaN comes before everything).
+//
+// A row is cut in slices, one for each CTA, when there are few rows; the last
+// CTA of a row joins them.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -39,7 +48,7 @@ struct Args {
   float* entropy;
   int* top_ids;
   float* top_lp;
-  float* part;  // [R][slices][4 + 2 * kMaxTop]
+  float* part;  // [R][slices][4 + 2 * kMaxTop]: m, r, S, W, keys
   int* counters;
 };
 
@@ -104,19 +113,40 @@ __device__ __forceinline__ Key block_merge(Key v, Key* lists) {
   return lists[lane];
 }
 
+// Running sums in the frame r; m is the largest value so far.
 struct Stat {
-  float m, s, w;
+  float m, r, s, w;
 };
-// Joins two running sums; m may be -inf (nothing but -inf so far).
+constexpr float kLowest = -1e30f;  // r of a thread without a finite value
+constexpr float kHuge = 1e29f;
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 __device__ __forceinline__ Stat join(const Stat& a, const Stat& b) {
-  Stat r;
-  r.m = max_nan(a.m, b.m);
-  const float ref = fmaxf(r.m, -FLT_MAX);
-  const float da = fmaxf(a.m, -FLT_MAX) - ref, db = fmaxf(b.m, -FLT_MAX) - ref;
-  const float fa = exp2f(da * kLog2e), fb = exp2f(db * kLog2e);
-  r.s = a.s * fa + b.s * fb;
-  r.w = (fa > 0.f ? fa * (a.w + a.s * da) : 0.f) + (fb > 0.f ? fb * (b.w + b.s * db) : 0.f);
-  return r;
+  Stat o;
+  o.m = max_nan(a.m, b.m);
+  o.r = fmaxf(a.r, b.r);
+  const float da = fmaxf(a.r - o.r, -200.f), db = fmaxf(b.r - o.r, -200.f);
+  const float fa = ex2(da), fb = ex2(db);
+  o.s = a.s * fa + b.s * fb;
+  o.w = fa * fmaf(a.s, da, a.w) + fb * fmaf(b.s, db, b.w);
+  return o;
+}
+__device__ __forceinline__ Stat warp_join(Stat v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    Stat u;
+    u.m = __shfl_xor_sync(0xffffffffu, v.m, o);
+    u.r = __shfl_xor_sync(0xffffffffu, v.r, o);
+    u.s = __shfl_xor_sync(0xffffffffu, v.s, o);
+    u.w = __shfl_xor_sync(0xffffffffu, v.w, o);
+    v = join(v, u);
+  }
+  return v;
 }
 
 template <typename T>
@@ -152,6 +182,7 @@ struct Chunk {
 template <typename T>
 __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const Args a) {
   constexpr int N = Chunk<T>::N;
+  constexpr int U = 4;  // chunks in flight for each thread
   __shared__ Key lists[kThreads];
   __shared__ Key cand[kCand];
   __shared__ Stat stats[kWarps];
@@ -161,103 +192,125 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const Args a) 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int row = blockIdx.y, slice = blockIdx.x;
   const T* x = reinterpret_cast<const T*>(a.x) + (int64_t)row * a.ld;
-  const int lo = slice * a.slice_len, hi = min(a.V, lo + a.slice_len);
+  const int lo = min(a.V, slice * a.slice_len), hi = min(a.V, lo + a.slice_len);
   // [lo, v0): before the first 16-byte boundary; [v0, v1): whole chunks.
   const int skew = (int)((reinterpret_cast<uintptr_t>(x + lo) & 15) / sizeof(T));
   const int v0 = min(hi, lo + (skew ? N - skew : 0));
   const int chunks = (hi - v0) / N;
   const int v1 = v0 + chunks * N;
   const uint4* xv = reinterpret_cast<const uint4*>(x + v0);
+  if (tid == 0) s_count = 0;
 
-  Stat st = {-INFINITY, 0.f, 0.f};
-  float ref = -FLT_MAX;
-  auto raise = [&](float to) {
-    const float n = fmaxf(to, -FLT_MAX);
-    const float d = ref - n;
-    const float f = exp2f(d * kLog2e);
-    st.w = f > 0.f ? f * (st.w + st.s * d) : 0.f;
+  Stat st = {-INFINITY, kLowest, 0.f, 0.f};
+  int best = tid;  // chunk of the largest value among the chunks
+  float best_v = -INFINITY;
+  bool nan = false;
+  auto raise = [&](float top) {
+    const float r = top * kLog2e;
+    const float d = fmaxf(st.r - r, -200.f);
+    const float f = ex2(d);
+    st.w = f * fmaf(st.s, d, st.w);
     st.s *= f;
-    st.m = max_nan(st.m, to);
-    ref = n;
+    st.r = r;
   };
   auto add = [&](float v) {
-    const float d = fmaxf(v - ref, -1e4f);
-    const float e = exp2f(d * kLog2e);
+    const float d = fmaxf(fmaf(v, kLog2e, -st.r), -200.f);  // -inf: a weight of 0, not a NaN
+    const float e = ex2(d);
     st.s += e;
     st.w = fmaf(e, d, st.w);
   };
-  // Edges: fewer than 2 N elements, one for each of the first threads.
-  const int edge = tid < v0 - lo ? lo + tid : (tid - (v0 - lo) < hi - v1 ? v1 + tid - (v0 - lo) : -1);
-  float edge_v = -INFINITY;
-  if (edge >= 0) {
-    edge_v = value(x + edge);
-    if (!(edge_v <= st.m)) raise(edge_v);
-    add(edge_v);
-  }
-  for (int c = tid; c < chunks; c += kThreads) {
+  auto take = [&](const uint4& raw, int c) {
     Chunk<T> u;
-    u.set(__ldg(xv + c));
+    u.set(raw);
     float top = u.v[0];
 #pragma unroll
     for (int i = 1; i < N; ++i) top = max_nan(top, u.v[i]);
-    if (!(top <= st.m)) raise(top);
+    nan |= top != top;
+    if (top > best_v) {
+      best_v = top;
+      best = c;
+    }
+    if (top * kLog2e > st.r + 8.f && top < kHuge) raise(top);
 #pragma unroll
     for (int i = 0; i < N; ++i) add(u.v[i]);
+  };
+  // Edges: fewer than 2 N elements, one for each of the first threads.
+  const int n0 = v0 - lo;
+  const int edge = tid < n0 ? lo + tid : (tid - n0 < hi - v1 ? v1 + tid - n0 : -1);
+  float edge_v = -INFINITY;
+  if (edge >= 0) {
+    edge_v = value(x + edge);
+    nan |= edge_v != edge_v;
+    if (edge_v > kLowest && edge_v < kHuge) raise(edge_v);
+    add(edge_v);
   }
-  // Row statistics.
+  int c = tid;
+  for (; c + (U - 1) * kThreads < chunks; c += U * kThreads) {
+    uint4 raw[U];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    Stat other;
-    other.m = __shfl_xor_sync(0xffffffffu, st.m, o);
-    other.s = __shfl_xor_sync(0xffffffffu, st.s, o);
-    other.w = __shfl_xor_sync(0xffffffffu, st.w, o);
-    st = join(st, other);
+    for (int i = 0; i < U; ++i) raw[i] = __ldg(xv + c + i * kThreads);
+#pragma unroll
+    for (int i = 0; i < U; ++i) take(raw[i], c + i * kThreads);
   }
-  if (lane == 0) stats[warp] = st;
-  __syncthreads();
-  st = stats[0];
-  for (int w = 1; w < kWarps; ++w) st = join(st, stats[w]);
+  {
+    uint4 raw[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      if (c + i * kThreads < chunks) raw[i] = __ldg(xv + c + i * kThreads);
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      if (c + i * kThreads < chunks) take(raw[i], c + i * kThreads);
+  }
+  st.m = nan ? __int_as_float(0x7fc00000) : fmaxf(best_v, edge_v);
 
+  // This thread's largest value with its index.
+  Key key = 0;
+  auto chunk_keys = [&](int at, auto&& use) {
+    Chunk<T> u;
+    u.set(__ldg(xv + at));
+#pragma unroll
+    for (int i = 0; i < N; ++i) use(make_key(u.v[i], v0 + at * N + i));
+  };
+  auto keep_largest = [&](Key k2) { key = k2 > key ? k2 : key; };
+  if (a.top_k > 0) {
+    if (edge >= 0) key = make_key(edge_v, edge);
+    if (nan) {
+      for (int i = tid; i < chunks; i += kThreads) chunk_keys(i, keep_largest);
+    } else if (best < chunks) {
+      chunk_keys(best, keep_largest);
+    }
+  }
+
+  st = warp_join(st);
+  if (lane == 0) stats[warp] = st;
   Key top = 0;
   if (a.top_k > 0) {
-    Key key = edge >= 0 ? make_key(edge_v, edge) : 0;
-    for (int c = tid; c < chunks; c += kThreads) {
-      Chunk<T> u;
-      u.set(__ldg(xv + c));
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const Key k2 = make_key(u.v[i], v0 + c * N + i);
-        key = k2 > key ? k2 : key;
+    const Key largest = block_merge(warp_sort(key), lists);
+    const Key bound = __shfl_sync(0xffffffffu, largest, a.top_k - 1);
+    auto offer = [&](Key k2) {
+      if (k2 >= bound && k2 > 0) {
+        const int at = atomicAdd(&s_count, 1);
+        if (at < kCand) cand[at] = k2;
       }
-    }
-    const Key bound_list = block_merge(warp_sort(key), lists);
-    const Key bound = __shfl_sync(0xffffffffu, bound_list, a.top_k - 1);
-    if (tid == 0) s_count = 0;
-    __syncthreads();
-    if (key >= bound && key > 0) {
-      if (edge >= 0) {
-        const Key k2 = make_key(edge_v, edge);
-        if (k2 >= bound) {
-          const int at = atomicAdd(&s_count, 1);
-          if (at < kCand) cand[at] = k2;
-        }
-      }
-      for (int c = tid; c < chunks; c += kThreads) {
-        Chunk<T> u;
-        u.set(__ldg(xv + c));
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const Key k2 = make_key(u.v[i], v0 + c * N + i);
-          if (k2 >= bound) {
-            const int at = atomicAdd(&s_count, 1);
-            if (at < kCand) cand[at] = k2;
-          }
-        }
-      }
+    };
+    if (edge >= 0) offer(make_key(edge_v, edge));
+    // The chunks of thread number j of the list, by one warp.
+    for (int j = warp; j < a.top_k; j += kWarps) {
+      const Key kj = __shfl_sync(0xffffffffu, largest, j);
+      if (kj == 0) break;
+      const int i = (int)~(uint32_t)kj;
+      const int owner = i < v0 ? i - lo : (i >= v1 ? n0 + i - v1 : ((i - v0) / N) % kThreads);
+      for (int at = owner + lane * kThreads; at < chunks; at += 32 * kThreads)
+        chunk_keys(at, offer);
     }
     __syncthreads();
     const int count = s_count;
-    if (count <= kCand) {
+    if (count <= 128) {
+      if (warp == 0) {
+        for (int i = 0; i < count; i += 32)
+          top = warp_merge(top, warp_sort(i + lane < count ? cand[i + lane] : 0));
+      }
+    } else if (count <= kCand) {
       for (int i = warp * 32; i < count; i += kThreads)
         top = warp_merge(top, warp_sort(i + lane < count ? cand[i + lane] : 0));
       top = block_merge(top, lists);
@@ -266,34 +319,29 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const Args a) 
       // largest values in a few threads' chunks): one pass for each place.
       Key last = ~(Key)0;
       for (int j = 0; j < a.top_k; ++j) {
-        Key k1 = edge >= 0 ? make_key(edge_v, edge) : 0;
-        if (k1 >= last) k1 = 0;
-        for (int c = tid; c < chunks; c += kThreads) {
-          Chunk<T> u;
-          u.set(__ldg(xv + c));
-#pragma unroll
-          for (int i = 0; i < N; ++i) {
-            const Key k2 = make_key(u.v[i], v0 + c * N + i);
-            if (k2 < last && k2 > k1) k1 = k2;
-          }
-        }
-        const Key found = block_merge(warp_sort(k1), lists);
+        key = edge >= 0 ? make_key(edge_v, edge) : 0;
+        if (key >= last) key = 0;
+        for (int i = tid; i < chunks; i += kThreads)
+          chunk_keys(i, [&](Key k2) { key = k2 < last && k2 > key ? k2 : key; });
+        const Key found = block_merge(warp_sort(key), lists);
         last = __shfl_sync(0xffffffffu, found, 0);
         if (lane == j) top = last;
       }
     }
+  } else {
+    __syncthreads();
+  }
+  if (warp == 0) {
+    st = lane < kWarps ? stats[lane] : Stat{-INFINITY, kLowest, 0.f, 0.f};
+    st = warp_join(st);
   }
 
   if (a.slices > 1) {
     constexpr int P = 4 + 2 * kMaxTop;
     float* part = a.part + ((int64_t)row * a.slices + slice) * P;
     if (warp == 0) {
-      if (lane == 0) {
-        part[0] = st.m;
-        part[1] = st.s;
-        part[2] = st.w;
-      }
-      reinterpret_cast<Key*>(part + 4)[lane] = top;
+      if (lane == 0) *reinterpret_cast<float4*>(part) = make_float4(st.m, st.r, st.s, st.w);
+      if (lane < a.top_k) reinterpret_cast<Key*>(part + 4)[lane] = top;
       __threadfence();
       __syncwarp();
       if (lane == 0) {
@@ -304,30 +352,61 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const Args a) 
     __syncthreads();
     if (!s_last) return;
     __threadfence();
-    if (warp == 0) {
-      st = {-INFINITY, 0.f, 0.f};
+    const float* parts = a.part + (int64_t)row * a.slices * P;
+    if (a.top_k > 0) {
       top = 0;
-      for (int i = 0; i < a.slices; ++i) {
-        const float* p = a.part + ((int64_t)row * a.slices + i) * P;
-        const Stat o = {__ldcg(p), __ldcg(p + 1), __ldcg(p + 2)};
-        st = join(st, o);
-        if (a.top_k > 0)
-          top = warp_merge(top, __ldcg(reinterpret_cast<const Key*>(p + 4) + lane));
+      for (int i = warp; i < a.slices; i += kWarps) {
+        const Key* p = reinterpret_cast<const Key*>(parts + i * P + 4);
+        top = warp_merge(top, lane < a.top_k ? __ldcg(p + lane) : 0);
       }
+      top = block_merge(top, lists);
+    }
+    if (warp == 0) {
+      st = {-INFINITY, kLowest, 0.f, 0.f};
+      for (int i = lane; i < a.slices; i += 32) {
+        const float4 f = __ldcg(reinterpret_cast<const float4*>(parts + i * P));
+        st = join(st, Stat{f.x, f.y, f.z, f.w});
+      }
+      st = warp_join(st);
     }
   }
-  if (warp != 0) return;
+
+  // From here on warp 0 holds the row's sums and list.
+  if (warp == 0 && lane == 0) stats[0] = st;
+  __syncthreads();
+  const float m = stats[0].m;
   // NaN or +inf in the row: no distribution.  Nothing but -inf: every token
   // has probability 0.
-  const bool bad = !(st.m < INFINITY);
-  const bool empty = st.m == -INFINITY;
-  const float ln_s = logf(st.s);
-  const float nan = __int_as_float(0x7fc00000);
-  auto lp_of = [&](float v) { return bad ? nan : (empty ? -INFINITY : (v - st.m) - ln_s); };
+  const bool bad = !(m < INFINITY), empty = m == -INFINITY;
+  const bool far = !bad && !empty && fabsf(m) >= kHuge;
+  if (far) {
+    int same = 0;
+    for (int i = tid; i < a.V; i += kThreads) same += value(x + i) == m;
+    same = __reduce_add_sync(0xffffffffu, same);
+    if (lane == 0) lists[warp] = same;
+    __syncthreads();
+    if (tid == 0) {
+      Key total = 0;
+      for (int w = 0; w < kWarps; ++w) total += lists[w];
+      stats[0] = Stat{m, 0.f, (float)total, 0.f};
+    }
+    __syncthreads();
+    st = stats[0];
+  }
+  if (warp != 0) return;
+  constexpr float kLn2 = 0.6931471805599453f;
+  const float log2_s = log2f(st.s);
+  const float none = __int_as_float(0x7fc00000);
+  auto lp_of = [&](float v) {
+    if (bad) return none;
+    if (empty || v == -INFINITY) return -INFINITY;
+    if (far || fabsf(v) >= kHuge) return (v - m) - log2_s * kLn2;  // v log2e may overflow
+    return (fmaf(v, kLog2e, -st.r) - log2_s) * kLn2;
+  };
   if (lane == 0) {
     const int t = a.tokens[row];
-    a.logprob[row] = t >= 0 && t < a.V ? lp_of(value(x + t)) : nan;
-    a.entropy[row] = bad ? nan : (empty ? 0.f : ln_s - st.w / st.s);
+    a.logprob[row] = t >= 0 && t < a.V ? lp_of(value(x + t)) : none;
+    a.entropy[row] = bad ? none : (empty ? 0.f : (log2_s - st.w / st.s) * kLn2);
   }
   if (lane < a.top_k) {
     a.top_ids[(int64_t)row * a.top_k + lane] = (int)~(uint32_t)top;
@@ -339,8 +418,8 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const Args a) 
 
 // {slices of a row, workspace floats, workspace counters} of token_logprobs.
 std::vector<int64_t> token_logprobs_plan(int64_t rows, int64_t vocab, int64_t elem_size) {
-  // About four CTAs for each SM, slices of two chunks a thread at least.
-  const int64_t least = 2 * lp::kThreads * (16 / elem_size);
+  // About four CTAs for each SM, slices of one chunk a thread at least.
+  const int64_t least = lp::kThreads * (16 / elem_size);
   int64_t s = std::max<int64_t>(1, 4 * num_sms() / std::max<int64_t>(1, rows));
   s = std::min(s, std::max<int64_t>(1, vocab / least));
   return {s, s > 1 ? rows * s * (4 + 2 * lp::kMaxTop) : 0, s > 1 ? rows : 0};
