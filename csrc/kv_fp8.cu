@@ -76,7 +76,10 @@ __device__ __forceinline__ uint2 pack8_e4m3(const float (&v)[8], float inv) {
 // D / 16 lanes share one head row; each holds two chunks of 8 values: the two
 // halves of 8 rotation pairs (half layout), or 16 neighbours (interleaved
 // pairs, and everything that is not rotated).
-template <int D>
+// A thread handles HPT heads of its token, all loaded before the first is used
+// (and before the cosines arrive); with few tokens the heads of a token spread
+// over gridDim.y CTAs instead.
+template <int D, int HPT>
 __global__ void __launch_bounds__(128) rope_kv_write_fp8_kernel(const WriteArgs a) {
   constexpr int LPH = D / 16;
   constexpr int GROUPS = 128 / LPH;
@@ -90,49 +93,57 @@ __global__ void __launch_bounds__(128) rope_kv_write_fp8_kernel(const WriteArgs 
   const bool split = rotated && !a.interleaved;
   const int d0 = split ? 8 * p : 16 * p;
   const int d1 = split ? half + 8 * p : 16 * p + 8;
-  float c[8], sn[8];
+  const int heads = a.Hq + 2 * a.Hkv;
+  const bf16* row = a.qkv + (int64_t)t * a.ldq;
+  const int h0 = blockIdx.y * HPT * GROUPS + threadIdx.x / LPH;
+  uint4 raw[HPT][2];
+#pragma unroll
+  for (int k = 0; k < HPT; ++k) {
+    const int h = h0 + k * GROUPS;
+    if (h < heads) {
+      raw[k][0] = *reinterpret_cast<const uint4*>(row + (int64_t)h * D + d0);
+      raw[k][1] = *reinterpret_cast<const uint4*>(row + (int64_t)h * D + d1);
+    } else {
+      raw[k][0] = raw[k][1] = make_uint4(0u, 0u, 0u, 0u);
+    }
+  }
+  alignas(16) float c[8], sn[8];
   if (rotated) {
     const float* cs = a.cos_sin + (int64_t)a.positions[t] * a.rot + 8 * p;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      c[i] = cs[i];
-      sn[i] = cs[half + i];
+    for (int i = 0; i < 8; i += 4) {
+      *reinterpret_cast<float4*>(c + i) = __ldg(reinterpret_cast<const float4*>(cs + i));
+      *reinterpret_cast<float4*>(sn + i) = __ldg(reinterpret_cast<const float4*>(cs + half + i));
     }
   }
-  const int heads = a.Hq + 2 * a.Hkv;
-  const bf16* row = a.qkv + (int64_t)t * a.ldq;
-  for (int hb = blockIdx.y * GROUPS; hb < heads; hb += gridDim.y * GROUPS) {
-    const int h = hb + threadIdx.x / LPH;
+#pragma unroll
+  for (int k = 0; k < HPT; ++k) {
+    const int h = h0 + k * GROUPS;
     const bool live = h < heads && (h < a.Hq || slot >= 0);
     float y0[8], y1[8];
-    if (live) {
-      unpack8(*reinterpret_cast<const uint4*>(row + (int64_t)h * D + d0), y0);
-      unpack8(*reinterpret_cast<const uint4*>(row + (int64_t)h * D + d1), y1);
-      if (rotated && h < a.Hq + a.Hkv) {
-        // Products and sums are rounded one by one (no contraction), so that
-        // codes do not depend on how the compiler fuses them.
-        if (a.interleaved) {
+    unpack8(raw[k][0], y0);
+    unpack8(raw[k][1], y1);
+    if (rotated && h < a.Hq + a.Hkv) {
+      // Products and sums are rounded one by one (no contraction), so that
+      // codes do not depend on how the compiler fuses them.
+      if (a.interleaved) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float u0 = y0[2 * i], u1 = y0[2 * i + 1];
-            y0[2 * i] = __fsub_rn(__fmul_rn(u0, c[i]), __fmul_rn(u1, sn[i]));
-            y0[2 * i + 1] = __fadd_rn(__fmul_rn(u1, c[i]), __fmul_rn(u0, sn[i]));
-            const float w0 = y1[2 * i], w1 = y1[2 * i + 1];
-            y1[2 * i] = __fsub_rn(__fmul_rn(w0, c[4 + i]), __fmul_rn(w1, sn[4 + i]));
-            y1[2 * i + 1] = __fadd_rn(__fmul_rn(w1, c[4 + i]), __fmul_rn(w0, sn[4 + i]));
-          }
-        } else {
+        for (int i = 0; i < 4; ++i) {
+          const float u0 = y0[2 * i], u1 = y0[2 * i + 1];
+          y0[2 * i] = __fsub_rn(__fmul_rn(u0, c[i]), __fmul_rn(u1, sn[i]));
+          y0[2 * i + 1] = __fadd_rn(__fmul_rn(u1, c[i]), __fmul_rn(u0, sn[i]));
+          const float w0 = y1[2 * i], w1 = y1[2 * i + 1];
+          y1[2 * i] = __fsub_rn(__fmul_rn(w0, c[4 + i]), __fmul_rn(w1, sn[4 + i]));
+          y1[2 * i + 1] = __fadd_rn(__fmul_rn(w1, c[4 + i]), __fmul_rn(w0, sn[4 + i]));
+        }
+      } else {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float u0 = y0[i], u1 = y1[i];
-            y0[i] = __fsub_rn(__fmul_rn(u0, c[i]), __fmul_rn(u1, sn[i]));
-            y1[i] = __fadd_rn(__fmul_rn(u1, c[i]), __fmul_rn(u0, sn[i]));
-          }
+        for (int i = 0; i < 8; ++i) {
+          const float u0 = y0[i], u1 = y1[i];
+          y0[i] = __fsub_rn(__fmul_rn(u0, c[i]), __fmul_rn(u1, sn[i]));
+          y1[i] = __fadd_rn(__fmul_rn(u1, c[i]), __fmul_rn(u0, sn[i]));
         }
       }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) y0[i] = y1[i] = 0.f;
     }
     // Largest magnitude over the row's lanes, on the bit patterns: an infinity
     // or a NaN is larger than every finite value.
@@ -172,50 +183,65 @@ __global__ void __launch_bounds__(128) rope_kv_write_fp8_kernel(const WriteArgs 
 }
 
 struct ReadArgs {
-  const uint8_t* code[2];  // K, V
-  const float* scale[2];
-  bf16* out[2];  // [N, Hkv, 16, D]
+  const uint8_t* k;
+  const uint8_t* v;
+  const float* ks;
+  const float* vs;
+  bf16* k_out;  // [N, Hkv, 16, D]
+  bf16* v_out;
   const int* blocks;
   int64_t layer_blocks;
-  int64_t chunks;  // 16-code chunks of one output
-  int per_block;   // chunks of one block: Hkv * 16 * D / 16
+  uint32_t items;      // 8-code pieces of K and V together: 2 N per_block
+  uint32_t per_block;  // pieces of one block of one of them: Hkv * 16 * D / 8
 };
 
-// One thread turns 16 codes of one row into 16 bf16 values.
+// A thread turns pieces of 8 codes into 8 bf16 values each: 8-byte loads and
+// 16-byte stores, both whole lines for a warp, and kReadPieces of them in
+// flight.  Pieces run over [block][K, V][head][token][dim].
+constexpr int kReadPieces = 8;
+
 template <int D>
 __global__ void __launch_bounds__(256) kv_read_fp8_kernel(const ReadArgs a) {
   grid_dep_launch();
   grid_dep_wait();
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= a.chunks) return;
-  const int w = blockIdx.y;
-  const int64_t n = i / a.per_block;
-  const int c = (int)(i - n * a.per_block);
-  const int blk = a.blocks[n];
-  uint4 out[2] = {make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)};
-  if (blk >= 0) {
-    const int64_t src = (a.layer_blocks + blk) * a.per_block + c;
-    const uint4 u = reinterpret_cast<const uint4*>(a.code[w])[src];
-    const float s = a.scale[w][src / (D / 16)];
-    const uint32_t x[4] = {u.x, u.y, u.z, u.w};
+  const uint32_t base = blockIdx.x * (256 * kReadPieces) + threadIdx.x;
+  uint2 code[kReadPieces];
+  float scale[kReadPieces];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      float y[8];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const __nv_fp8x2_storage_t pair =
-            (__nv_fp8x2_storage_t)(x[2 * k + j / 2] >> (16 * (j & 1)));
-        const __half2 h2 = __nv_cvt_fp8x2_to_halfraw2(pair, __NV_E4M3);
-        const float2 f = __half22float2(h2);
-        y[2 * j] = f.x * s;
-        y[2 * j + 1] = f.y * s;
+  for (int j = 0; j < kReadPieces; ++j) {
+    const uint32_t i = base + j * 256;
+    code[j] = make_uint2(0u, 0u);
+    scale[j] = 0.f;
+    if (i < a.items) {
+      const uint32_t pair = i / a.per_block;
+      const uint32_t c = i - pair * a.per_block;
+      const int blk = a.blocks[pair >> 1];
+      if (blk >= 0) {
+        const int64_t src = (a.layer_blocks + blk) * a.per_block + c;
+        code[j] = __ldg(reinterpret_cast<const uint2*>(pair & 1 ? a.v : a.k) + src);
+        scale[j] = __ldg((pair & 1 ? a.vs : a.ks) + src / (D / 8));
       }
-      out[k] = pack8_bf16(y);
     }
   }
-  uint4* dst = reinterpret_cast<uint4*>(a.out[w]) + 2 * i;
-  dst[0] = out[0];
-  dst[1] = out[1];
+#pragma unroll
+  for (int j = 0; j < kReadPieces; ++j) {
+    const uint32_t i = base + j * 256;
+    if (i >= a.items) continue;
+    const uint32_t pair = i / a.per_block;
+    const uint32_t c = i - pair * a.per_block;
+    float y[8];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const uint32_t word = w < 2 ? code[j].x : code[j].y;
+      const __half2 h2 = __nv_cvt_fp8x2_to_halfraw2(
+          (__nv_fp8x2_storage_t)(word >> (16 * (w & 1))), __NV_E4M3);
+      const float2 f = __half22float2(h2);
+      y[2 * w] = f.x * scale[j];
+      y[2 * w + 1] = f.y * scale[j];
+    }
+    uint4* dst = reinterpret_cast<uint4*>(pair & 1 ? a.v_out : a.k_out);
+    dst[(int64_t)(pair >> 1) * a.per_block + c] = pack8_bf16(y);
+  }
 }
 
 // ---------------------------------------------------------------- host side
@@ -235,6 +261,21 @@ static void check_fp8_cache(const torch::Tensor& k, const torch::Tensor& v,
               "k/v scales must be fp32 [L, NB, Hkv, 16] contiguous");
   TORCH_CHECK(v.device() == k.device() && ks.device() == k.device() && vs.device() == k.device(),
               "cache and scales must be on one device");
+}
+
+// Few tokens: one head a thread, so that the heads' loads and the row maxima of
+// one token run side by side; from four CTAs an SM on, three heads a thread.
+template <int D>
+static void launch_write(const WriteArgs& a, cudaStream_t stream) {
+  constexpr int groups = 128 / (D / 16);
+  const int heads = a.Hq + 2 * a.Hkv;
+  if (a.T < 4 * num_sms()) {
+    const dim3 grid((unsigned)a.T, (heads + groups - 1) / groups);
+    launch_kernel(rope_kv_write_fp8_kernel<D, 1>, grid, dim3(128), 0, stream, a);
+  } else {
+    const dim3 grid((unsigned)a.T, (heads + 3 * groups - 1) / (3 * groups));
+    launch_kernel(rope_kv_write_fp8_kernel<D, 3>, grid, dim3(128), 0, stream, a);
+  }
 }
 
 void rope_kv_write_fp8(torch::Tensor qkv, torch::Tensor positions, torch::Tensor cos_sin,
@@ -264,8 +305,9 @@ void rope_kv_write_fp8(torch::Tensor qkv, torch::Tensor positions, torch::Tensor
               "q_out must be bf16 [T, Hq D] with inner stride 1");
   TORCH_CHECK((qkv.stride(0) * 2) % 16 == 0 && (qo.stride(0) * 2) % 16 == 0 &&
                   reinterpret_cast<uintptr_t>(qkv.data_ptr()) % 16 == 0 &&
-                  reinterpret_cast<uintptr_t>(qo.data_ptr()) % 16 == 0,
-              "qkv / q_out rows must be 16-byte aligned");
+                  reinterpret_cast<uintptr_t>(qo.data_ptr()) % 16 == 0 &&
+                  reinterpret_cast<uintptr_t>(cos_sin.data_ptr()) % 16 == 0,
+              "qkv / q_out rows and cos_sin must be 16-byte aligned");
   TORCH_CHECK(qkv.device() == k_cache.device() && qo.device() == qkv.device() &&
                   positions.device() == qkv.device() && slots.device() == qkv.device() &&
                   cos_sin.device() == qkv.device(),
@@ -290,11 +332,10 @@ void rope_kv_write_fp8(torch::Tensor qkv, torch::Tensor positions, torch::Tensor
   a.Hkv = (int)Hkv;
   a.rot = (int)rot;
   a.interleaved = interleaved ? 1 : 0;
-  const dim3 grid((unsigned)T, 1);
   cudaStream_t stream = at::cuda::getCurrentCUDAStream();
-  if (D == 64) launch_kernel(rope_kv_write_fp8_kernel<64>, grid, dim3(128), 0, stream, a);
-  else if (D == 128) launch_kernel(rope_kv_write_fp8_kernel<128>, grid, dim3(128), 0, stream, a);
-  else launch_kernel(rope_kv_write_fp8_kernel<256>, grid, dim3(128), 0, stream, a);
+  if (D == 64) launch_write<64>(a, stream);
+  else if (D == 128) launch_write<128>(a, stream);
+  else launch_write<256>(a, stream);
 }
 
 void kv_read_fp8(torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor k_scale,
@@ -317,23 +358,26 @@ void kv_read_fp8(torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor k_s
   if (N == 0) return;
   const c10::cuda::CUDAGuard guard(k_cache.device());
   ReadArgs a;
-  a.code[0] = reinterpret_cast<const uint8_t*>(k_cache.data_ptr());
-  a.code[1] = reinterpret_cast<const uint8_t*>(v_cache.data_ptr());
-  a.scale[0] = k_scale.data_ptr<float>();
-  a.scale[1] = v_scale.data_ptr<float>();
-  a.out[0] = reinterpret_cast<bf16*>(k_out.data_ptr());
-  a.out[1] = reinterpret_cast<bf16*>(v_out.data_ptr());
-  a.blocks = blocks.data_ptr<int>();
+  a.k = reinterpret_cast<const uint8_t*>(k_cache.data_ptr());
+  a.v = reinterpret_cast<const uint8_t*>(v_cache.data_ptr());
+  a.ks = k_scale.data_ptr<float>();
+  a.vs = v_scale.data_ptr<float>();
   a.layer_blocks = layer * k_cache.size(1);
-  a.per_block = (int)(Hkv * D);
-  a.chunks = N * a.per_block;
-  const int64_t ctas = (a.chunks + 255) / 256;
-  TORCH_CHECK(ctas < (int64_t(1) << 31), "too many blocks for one call");
-  const dim3 grid((unsigned)ctas, 2);
+  a.per_block = (uint32_t)(Hkv * 2 * D);
   cudaStream_t stream = at::cuda::getCurrentCUDAStream();
-  if (D == 64) launch_kernel(kv_read_fp8_kernel<64>, grid, dim3(256), 0, stream, a);
-  else if (D == 128) launch_kernel(kv_read_fp8_kernel<128>, grid, dim3(256), 0, stream, a);
-  else launch_kernel(kv_read_fp8_kernel<256>, grid, dim3(256), 0, stream, a);
+  // Pieces are counted in 32 bits: a call past that is cut into several launches.
+  const int64_t most = ((int64_t(1) << 31) - 1) / (2 * a.per_block);
+  for (int64_t n0 = 0; n0 < N; n0 += most) {
+    const int64_t n = std::min(most, N - n0);
+    a.k_out = reinterpret_cast<bf16*>(k_out.data_ptr()) + n0 * Hkv * 16 * D;
+    a.v_out = reinterpret_cast<bf16*>(v_out.data_ptr()) + n0 * Hkv * 16 * D;
+    a.blocks = blocks.data_ptr<int>() + n0;
+    a.items = (uint32_t)(2 * n * a.per_block);
+    const dim3 grid((a.items + 256 * kReadPieces - 1) / (256 * kReadPieces));
+    if (D == 64) launch_kernel(kv_read_fp8_kernel<64>, grid, dim3(256), 0, stream, a);
+    else if (D == 128) launch_kernel(kv_read_fp8_kernel<128>, grid, dim3(256), 0, stream, a);
+    else launch_kernel(kv_read_fp8_kernel<256>, grid, dim3(256), 0, stream, a);
+  }
 }
 
 }  // namespace cb
