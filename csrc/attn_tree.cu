@@ -81,6 +81,19 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Transpose of an 8 x 8 matrix of 16-bit values held two to a lane.
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
 // Streaming load: a cache row is read once by one SM.
 __device__ __forceinline__ uint4 ldg_stream16(const void* p) {
   uint4 v;
@@ -146,15 +159,14 @@ struct Block {
   static constexpr int VW = FP8 ? D / 32 : D / 16;  // V words of a lane and token
   uint4 k[2][KC];
   uint32_t v[4][VW];
-  float2 ks[2], vs[2];
+  float ks[2], vs[2];
 
-  // Tokens of lane (g, t4): K rows g and 8 + g; V rows 2 t4, 2 t4 + 1 and
-  // those plus 8.  A lane's K chunk c holds the head dims of its k-steps (any
-  // order of the summed dims will do, if q has the same), its V words the
-  // D / 8 dims from g D / 8 on.
-  __device__ __forceinline__ void load(const Args& a, const int* table, int h, int blk, int g,
-                                       int t4) {
-    const int64_t row = ((a.layer_blocks + table[blk]) * a.Hkv + h) * 16;
+  // Tokens of lane (g, t4): K rows g and 8 + g (their scales too); V rows
+  // 2 t4, 2 t4 + 1 and those plus 8.  A lane's K chunk c holds the head dims of
+  // its k-steps (any order of the summed dims will do, if q has the same), its
+  // V words the D / 8 dims from g D / 8 on.
+  __device__ __forceinline__ void load(const Args& a, int page, int h, int g, int t4) {
+    const int64_t row = ((a.layer_blocks + page) * a.Hkv + h) * 16;
     constexpr int RB = FP8 ? D : 2 * D;  // bytes of a row
     const uint8_t* kp = a.k + row * RB;
     const uint8_t* vp = a.v + row * RB;
@@ -165,8 +177,8 @@ struct Block {
     if constexpr (FP8) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        ks[i] = *reinterpret_cast<const float2*>(a.ks + row + 8 * i + 2 * t4);
-        vs[i] = *reinterpret_cast<const float2*>(a.vs + row + 8 * i + 2 * t4);
+        ks[i] = __ldg(a.ks + row + 8 * i + g);
+        vs[i] = __ldg(a.vs + row + 8 * i + g);
       }
     }
 #pragma unroll
@@ -190,19 +202,213 @@ struct Block {
   }
 };
 
-// 4 warps; each takes every fourth block of a job's keys for all 16 rows of the
+// What a warp carries through a job's keys for NR x 8 query rows.  Products are
+// taken transposed, S^T = K q^T and O^T = V^T P^T, so that the keys fill the 16
+// rows of the warp-level product and the query rows its 8 columns: a single
+// token's group of up to 8 heads wastes nothing.
+template <int D, bool FP8, int NR>
+struct Warp {
+  static constexpr int NKS = D / 16;
+  static constexpr int NT = D / 8;
+  uint32_t q[NR][NKS][2];
+  float row_scale[NR][2];
+  int node[NR][2];  // of score columns 2 t4, 2 t4 + 1
+  float o[NR][NT / 2][4];
+  float m[NR][2], l[NR][2];
+
+  __device__ __forceinline__ bool sees(const Args& a, int n, int e, int j, int q_row0) const {
+    if (a.masks == nullptr) return j <= node[n][e];
+    return j < 64 && (__ldg(a.masks + q_row0 + node[n][e]) >> (j & 63) & 1);
+  }
+
+  __device__ __forceinline__ void step(const Args& a, Block<D, FP8>& x, int blk, int page, int h,
+                                       int len, int ctx, int q_row0, int g, int t4) {
+    const int pos0 = blk * 16;
+    float sc[NR][4];
+#pragma unroll
+    for (int n = 0; n < NR; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
+#pragma unroll
+    for (int c = 0; c < Block<D, FP8>::KC; ++c) {
+      const uint32_t w0[4] = {x.k[0][c].x, x.k[0][c].y, x.k[0][c].z, x.k[0][c].w};
+      const uint32_t w1[4] = {x.k[1][c].x, x.k[1][c].y, x.k[1][c].z, x.k[1][c].w};
+      if constexpr (FP8) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t kf[4] = {e4m3x2_to_f16x2(w0[i] & 0xffffu), e4m3x2_to_f16x2(w1[i] & 0xffffu),
+                                  e4m3x2_to_f16x2(w0[i] >> 16), e4m3x2_to_f16x2(w1[i] >> 16)};
+#pragma unroll
+          for (int n = 0; n < NR; ++n) mma_f16(sc[n], kf, q[n][4 * c + i][0], q[n][4 * c + i][1]);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t kf[4] = {w0[2 * i], w1[2 * i], w0[2 * i + 1], w1[2 * i + 1]};
+#pragma unroll
+          for (int n = 0; n < NR; ++n) mma_16816(sc[n], kf, q[n][2 * c + i][0], q[n][2 * c + i][1]);
+        }
+      }
+    }
+    // Scores in base 2 (tokens g and g + 8 x rows 2 t4 and 2 t4 + 1).
+    float inv_vs[2] = {1.f, 1.f};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float kk = 1.f, lv = 0.f;
+      if constexpr (FP8) {
+        kk = x.ks[i];
+        lv = __log2f(x.vs[i]);
+        inv_vs[i] = ex2(-lv);
+      }
+#pragma unroll
+      for (int n = 0; n < NR; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          sc[n][2 * i + e] = FP8 ? fmaf(sc[n][2 * i + e], kk * row_scale[n][e], lv)
+                                 : sc[n][2 * i + e] * row_scale[n][e];
+    }
+    const bool tail = pos0 + 16 > ctx;
+    if (tail) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int pos = pos0 + 8 * i + g;
+        // A NaN scale of a key that some rows do not see stays out of their sums.
+        if (pos >= len) inv_vs[i] = 0.f;
+#pragma unroll
+        for (int n = 0; n < NR; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if (pos >= len || (pos >= ctx && !sees(a, n, e, pos - ctx, q_row0)))
+              sc[n][2 * i + e] = -INFINITY;
+      }
+      // Value rows past the end may hold anything: a weight of zero does not
+      // remove a NaN from a product.
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (pos0 + 8 * (i >> 1) + 2 * t4 + (i & 1) >= len) {
+#pragma unroll
+          for (int w = 0; w < Block<D, FP8>::VW; ++w) x.v[i][w] = 0u;
+        }
+      if constexpr (!FP8) take_out_infinities(a, x, pos0, page, h, len, ctx, q_row0, g, t4);
+    }
+    uint32_t pf[NR][2];
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+      float p[4];
+      float alpha[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float mx = fmaxf(sc[n][e], sc[n][2 + e]);
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+        const float m_new = fmaxf(m[n][e], mx);
+        alpha[e] = ex2(m[n][e] - m_new);
+        const float base = FP8 ? m_new - 15.f : m_new;
+        m[n][e] = m_new;
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float w = ex2(sc[n][2 * i + e] - base);
+          p[2 * i + e] = w;
+          // (a hidden key's weight is 0: its scale, which may be a NaN, must
+          // not turn that into one)
+          if constexpr (FP8) sum += tail && w == 0.f ? 0.f : w * inv_vs[i];
+          else sum += w;
+        }
+        l[n][e] = fmaf(l[n][e], alpha[e], sum);
+      }
+      if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
+#pragma unroll
+        for (int i = 0; i < NT / 2; ++i) {
+          o[n][i][0] *= alpha[0];
+          o[n][i][1] *= alpha[1];
+          o[n][i][2] *= alpha[0];
+          o[n][i][3] *= alpha[1];
+        }
+      }
+      // Weights as the second operand: token pairs of one row a register.
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        pf[n][i] = transpose8(FP8 ? pack_f16(p[2 * i], p[2 * i + 1])
+                                  : pack_bf16(p[2 * i], p[2 * i + 1]));
+    }
+#pragma unroll
+    for (int w = 0; w < Block<D, FP8>::VW; ++w) {
+      if constexpr (FP8) {
+        // Bytes of two tokens side by side, four dims a word.
+        const uint32_t a0 = __byte_perm(x.v[0][w], x.v[1][w], 0x5140);
+        const uint32_t a1 = __byte_perm(x.v[0][w], x.v[1][w], 0x7362);
+        const uint32_t b0 = __byte_perm(x.v[2][w], x.v[3][w], 0x5140);
+        const uint32_t b1 = __byte_perm(x.v[2][w], x.v[3][w], 0x7362);
+        const uint32_t v0[4] = {e4m3x2_to_f16x2(a0 & 0xffffu), e4m3x2_to_f16x2(a0 >> 16),
+                                e4m3x2_to_f16x2(b0 & 0xffffu), e4m3x2_to_f16x2(b0 >> 16)};
+        const uint32_t v1[4] = {e4m3x2_to_f16x2(a1 & 0xffffu), e4m3x2_to_f16x2(a1 >> 16),
+                                e4m3x2_to_f16x2(b1 & 0xffffu), e4m3x2_to_f16x2(b1 >> 16)};
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+          mma_f16(o[n][2 * w], v0, pf[n][0], pf[n][1]);
+          mma_f16(o[n][2 * w + 1], v1, pf[n][0], pf[n][1]);
+        }
+      } else {
+        const uint32_t vf[4] = {__byte_perm(x.v[0][w], x.v[1][w], 0x5410),
+                                __byte_perm(x.v[0][w], x.v[1][w], 0x7632),
+                                __byte_perm(x.v[2][w], x.v[3][w], 0x5410),
+                                __byte_perm(x.v[2][w], x.v[3][w], 0x7632)};
+#pragma unroll
+        for (int n = 0; n < NR; ++n) mma_16816(o[n][w], vf, pf[n][0], pf[n][1]);
+      }
+    }
+  }
+
+  // A node may hold an infinity or a NaN that its siblings do not see: such
+  // values leave the product and are added to the rows that do.
+  __device__ __forceinline__ void take_out_infinities(const Args& a, Block<D, FP8>& x, int pos0,
+                                                      int page, int h, int len, int ctx,
+                                                      int q_row0, int g, int t4) {
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int w = 0; w < Block<D, FP8>::VW; ++w) {
+        uint32_t y = x.v[i][w];
+        if ((y & 0x7f80u) == 0x7f80u) { y &= 0xffff0000u; bad = true; }
+        if ((y & 0x7f800000u) == 0x7f800000u) { y &= 0xffffu; bad = true; }
+        x.v[i][w] = y;
+      }
+    if (!__any_sync(0xffffffffu, bad)) return;
+    const int64_t row = ((a.layer_blocks + page) * a.Hkv + h) * 16;
+    const __nv_bfloat16* vp = reinterpret_cast<const __nv_bfloat16*>(a.v) + row * D;
+    for (int tok = 0; tok < 16 && pos0 + tok < len; ++tok) {
+      const int j = pos0 + tok - ctx;
+#pragma unroll
+      for (int n = 0; n < NR; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          if (j >= 0 && !sees(a, n, e, j, q_row0)) continue;
+#pragma unroll
+          for (int i = 0; i < NT; ++i) {
+            const float val = __bfloat162float(vp[tok * D + g * NT + i]);
+            if (!(fabsf(val) <= 3.4e38f)) o[n][i / 2][2 * (i & 1) + e] += val;
+          }
+        }
+    }
+  }
+};
+
+// 4 warps; each takes every fourth block of a job's keys for all rows of the
 // job's tile and streams K and V from global memory straight into the operand
 // registers of its warp-level products (a row of 128 B is one whole line, and
-// no byte is used by two warps, so shared memory would only add a copy).
-template <int D, bool FP8>
-__global__ void __launch_bounds__(128) attn_rows_kernel(const Args a) {
-  constexpr int ROWS = 16;
+// no byte is used by two warps, so shared memory would only add a copy).  The
+// next block is in flight while one is worked on.
+template <int D, bool FP8, int NR>
+__global__ void __launch_bounds__(128, NR == 1 && FP8 ? 3 : 2) attn_rows_kernel(const Args a) {
+  constexpr int ROWS = 8 * NR;
   constexpr int NKS = D / 16;
   constexpr int NT = D / 8;
+  constexpr int LD = D + 4;  // row pitch of the joined sums in shared memory
   extern __shared__ __align__(16) uint8_t smem_raw[];
   int64_t* pre = reinterpret_cast<int64_t*>(smem_raw);
-  float* sm_o = reinterpret_cast<float*>(smem_raw + ((a.B + 2) / 2 * 2) * 8);  // [4][16][D]
-  float* sm_ml = sm_o + 4 * ROWS * D;                                         // [4][16][2]
+  float* sm_o = reinterpret_cast<float*>(smem_raw + ((a.B + 2) / 2 * 2) * 8);  // [4][ROWS][LD]
+  float* sm_ml = sm_o + 4 * ROWS * LD;                                        // [4][ROWS][2]
   __shared__ int64_t s_sum[4];
   __shared__ int s_last;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -238,34 +444,36 @@ __global__ void __launch_bounds__(128) attn_rows_kernel(const Args a) {
     const int q_row0 = a.row_start[b];
     const int rows_left = s.n * a.G - tile * ROWS;
 
-    // The two rows of this lane (g and g + 8 of the tile).
-    int node[2];
-    uint64_t mask[2];
-    float row_scale[2];
-    uint32_t qa[NKS][4];
+    const int blk_end = min(k1, (s.len + 15) >> 4);
+    const int first = k0 + warp;
+    // Pages of this warp's blocks, 32 at a time, one in each lane.
+    int pages = first + 4 * lane < blk_end ? __ldg(table + first + 4 * lane) : 0;
+    Block<D, FP8> x[2];
+    if (first < blk_end) x[0].load(a, __shfl_sync(0xffffffffu, pages, 0), h, g, t4);
+
+    Warp<D, FP8, NR> w;
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int rr = tile * ROWS + g + 8 * r;
-      const bool live = g + 8 * r < rows_left;
-      node[r] = live ? rr / a.G : 0;
-      const int head = h * a.G + (live ? rr - node[r] * a.G : 0);
-      mask[r] = 0;
-      if (live && a.masks != nullptr) mask[r] = (uint64_t)a.masks[q_row0 + node[r]];
-      const __nv_bfloat16* qp = a.q + (int64_t)(q_row0 + node[r]) * a.q_stride + (int64_t)head * D;
+    for (int n = 0; n < NR; ++n) {
+      // Row 8 n + g as the second operand: dims in the K chunks' order.
+      const int r = 8 * n + g;
+      const bool live = r < rows_left;
+      const int rr = tile * ROWS + (live ? r : 0);
+      const __nv_bfloat16* qp = a.q + (int64_t)(q_row0 + rr / a.G) * a.q_stride +
+                                (int64_t)(h * a.G + rr % a.G) * D;
       uint32_t top = 0;
 #pragma unroll
       for (int ks = 0; ks < NKS; ++ks) {
         const int d = FP8 ? (ks >> 2) * 64 + t4 * 16 + (ks & 3) * 4
                           : (ks >> 1) * 32 + t4 * 8 + (ks & 1) * 4;
-        const uint2 w = live ? *reinterpret_cast<const uint2*>(qp + d) : make_uint2(0u, 0u);
-        qa[ks][r] = w.x;
-        qa[ks][2 + r] = w.y;
+        const uint2 y = live ? *reinterpret_cast<const uint2*>(qp + d) : make_uint2(0u, 0u);
+        w.q[n][ks][0] = y.x;
+        w.q[n][ks][1] = y.y;
         if constexpr (FP8) {
-          top = max(top, max(w.x & 0x7fffu, (w.x >> 16) & 0x7fffu));
-          top = max(top, max(w.y & 0x7fffu, (w.y >> 16) & 0x7fffu));
+          top = max(top, max(y.x & 0x7fffu, (y.x >> 16) & 0x7fffu));
+          top = max(top, max(y.y & 0x7fffu, (y.y >> 16) & 0x7fffu));
         }
       }
-      row_scale[r] = a.scale_log2;
+      float back = a.scale_log2;
       if constexpr (FP8) {
         // A power of two that puts the row's largest value into [2^14, 2^15):
         // what it moves below fp16's smallest value is under 2^-38 of that.
@@ -274,228 +482,83 @@ __global__ void __launch_bounds__(128) attn_rows_kernel(const Args a) {
         const int e = (int)(top >> 7);  // biased exponent
         const int sh = e == 0 || e == 255 ? 0 : min(100, 127 + 14 - e);
         const float up = __int_as_float((127 + sh) << 23);
-        row_scale[r] *= __int_as_float((127 - sh) << 23);
+        back *= __int_as_float((127 - sh) << 23);
 #pragma unroll
-        for (int ks = 0; ks < NKS; ++ks) {
+        for (int ks = 0; ks < NKS; ++ks)
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            const uint32_t w = qa[ks][2 * k + r];
-            qa[ks][2 * k + r] = pack_f16(__uint_as_float(w << 16) * up,
-                                         __uint_as_float(w & 0xffff0000u) * up);
+            const uint32_t y = w.q[n][ks][k];
+            w.q[n][ks][k] = pack_f16(__uint_as_float(y << 16) * up,
+                                     __uint_as_float(y & 0xffff0000u) * up);
           }
-        }
       }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        w.row_scale[n][e] = __shfl_sync(0xffffffffu, back, (2 * t4 + e) * 4);
+        const int c = 8 * n + 2 * t4 + e;
+        w.node[n][e] = (tile * ROWS + (c < rows_left ? c : 0)) / a.G;
+        w.m[n][e] = kNegBig;
+        w.l[n][e] = 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < NT / 2; ++i)
+        w.o[n][i][0] = w.o[n][i][1] = w.o[n][i][2] = w.o[n][i][3] = 0.f;
     }
 
-    float o[NT][4];
+    int idx = 0;
+    for (int blk = first; blk < blk_end; blk += 8) {
 #pragma unroll
-    for (int i = 0; i < NT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-    float m[2] = {kNegBig, kNegBig};
-    float l[2] = {0.f, 0.f};
-
-    const int blk_end = min(k1, (s.len + 15) >> 4);
-    Block<D, FP8> x;
-    for (int blk = k0 + warp; blk < blk_end; blk += 4) {
-      x.load(a, table, h, blk, g, t4);
-      const int pos0 = blk * 16;
-      float sc[2][4];
-#pragma unroll
-      for (int nt = 0; nt < 2; ++nt) {
-        sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
-#pragma unroll
-        for (int c = 0; c < Block<D, FP8>::KC; ++c) {
-          const uint32_t w[4] = {x.k[nt][c].x, x.k[nt][c].y, x.k[nt][c].z, x.k[nt][c].w};
-          if constexpr (FP8) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              mma_f16(sc[nt], qa[4 * c + i], e4m3x2_to_f16x2(w[i] & 0xffffu),
-                      e4m3x2_to_f16x2(w[i] >> 16));
-          } else {
-            mma_16816(sc[nt], qa[2 * c], w[0], w[1]);
-            mma_16816(sc[nt], qa[2 * c + 1], w[2], w[3]);
-          }
-        }
+      for (int half = 0; half < 2; ++half) {
+        const int cur = blk + 4 * half;
+        if (cur >= blk_end) break;
+        const int page = __shfl_sync(0xffffffffu, pages, idx & 31);
+        if (((idx + 1) & 31) == 0)
+          pages = cur + 4 + 4 * lane < blk_end ? __ldg(table + cur + 4 + 4 * lane) : 0;
+        ++idx;
+        if (cur + 4 < blk_end)
+          x[half ^ 1].load(a, __shfl_sync(0xffffffffu, pages, idx & 31), h, g, t4);
+        w.step(a, x[half], cur, page, h, s.len, ctx, q_row0, g, t4);
       }
-      // Scores in base 2, hidden keys at -inf.
-      float inv_vs[2][2];
-#pragma unroll
-      for (int nt = 0; nt < 2; ++nt) {
-        float kk[2] = {1.f, 1.f}, lv[2] = {0.f, 0.f};
-        inv_vs[nt][0] = inv_vs[nt][1] = 1.f;
-        if constexpr (FP8) {
-          kk[0] = x.ks[nt].x;
-          kk[1] = x.ks[nt].y;
-          lv[0] = __log2f(x.vs[nt].x);
-          lv[1] = __log2f(x.vs[nt].y);
-          inv_vs[nt][0] = exp2f(-lv[0]);
-          inv_vs[nt][1] = exp2f(-lv[1]);
-        }
-#pragma unroll
-        for (int r = 0; r < 2; ++r)
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-            sc[nt][2 * r + e] = sc[nt][2 * r + e] * (kk[e] * row_scale[r]) + lv[e];
-      }
-      uint32_t hidden = 0;  // bit 4 nt + 2 r + e of this lane's scores
-      if (pos0 + 16 > ctx) {
-#pragma unroll
-        for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-          for (int r = 0; r < 2; ++r)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int pos = pos0 + 8 * nt + 2 * t4 + e;
-              const int j = pos - ctx;
-              bool sees = pos < s.len;
-              if (j >= 0)
-                sees = sees && (a.masks != nullptr ? j < 64 && ((mask[r] >> (j & 63)) & 1)
-                                                   : j <= node[r]);
-              if (!sees) {
-                sc[nt][2 * r + e] = -INFINITY;
-                hidden |= 1u << (4 * nt + 2 * r + e);
-              }
-            }
-        // Value rows past the end may hold anything: a weight of zero does
-        // not remove a NaN from a product.
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (pos0 + 8 * (i >> 1) + 2 * t4 + (i & 1) >= s.len) {
-#pragma unroll
-            for (int w = 0; w < Block<D, FP8>::VW; ++w) x.v[i][w] = 0u;
-          }
-      }
-      float p[2][4];
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        float mx = fmaxf(fmaxf(sc[0][2 * r], sc[0][2 * r + 1]), fmaxf(sc[1][2 * r], sc[1][2 * r + 1]));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const float m_new = fmaxf(m[r], mx);
-        const float alpha = exp2f(m[r] - m_new);
-        const float base = FP8 ? m_new - 15.f : m_new;
-        float sum = 0.f;
-#pragma unroll
-        for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float w = exp2f(sc[nt][2 * r + e] - base);
-            // A NaN scale of a hidden key must not reach the sum either.
-            if (hidden >> (4 * nt + 2 * r + e) & 1) w = 0.f;
-            else sum += FP8 ? w * inv_vs[nt][e] : w;
-            p[nt][2 * r + e] = w;
-          }
-        l[r] = l[r] * alpha + sum;
-        m[r] = m_new;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          o[nt][2 * r] *= alpha;
-          o[nt][2 * r + 1] *= alpha;
-        }
-      }
-      uint32_t pa[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        pa[i] = FP8 ? pack_f16(p[i >> 1][2 * (i & 1)], p[i >> 1][2 * (i & 1) + 1])
-                    : pack_bf16(p[i >> 1][2 * (i & 1)], p[i >> 1][2 * (i & 1) + 1]);
-      if constexpr (!FP8) {
-        // A node may hold an infinity or a NaN that its siblings do not see:
-        // those values leave the product and are added to the rows that do.
-        if (pos0 + 16 > ctx) {
-          bool bad = false;
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int w = 0; w < Block<D, FP8>::VW; ++w) {
-              uint32_t y = x.v[i][w];
-              if ((y & 0x7f80u) == 0x7f80u) { y &= 0xffff0000u; bad = true; }
-              if ((y & 0x7f800000u) == 0x7f800000u) { y &= 0xffffu; bad = true; }
-              x.v[i][w] = y;
-            }
-          if (__any_sync(0xffffffffu, bad)) {
-            const int64_t row = ((a.layer_blocks + table[blk]) * a.Hkv + h) * 16;
-            const __nv_bfloat16* vp = reinterpret_cast<const __nv_bfloat16*>(a.v) + row * D;
-            for (int tok = 0; tok < 16 && pos0 + tok < s.len; ++tok) {
-              const int j = pos0 + tok - ctx;
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                  const float val = __bfloat162float(vp[tok * D + (2 * t4 + e) * NT + nt]);
-                  if (!(fabsf(val) <= 3.4e38f)) {
-#pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                      const bool sees =
-                          j < 0 || (a.masks != nullptr ? j < 64 && ((mask[r] >> (j & 63)) & 1)
-                                                       : j <= node[r]);
-                      if (sees) o[nt][2 * r + e] += val;
-                    }
-                  }
-                }
-            }
-          }
-        }
-      }
-#pragma unroll
-      for (int w = 0; w < Block<D, FP8>::VW; ++w) {
-        if constexpr (FP8) {
-          // Bytes of the two tokens side by side, four dims a word.
-          const uint32_t a0 = __byte_perm(x.v[0][w], x.v[1][w], 0x5140);
-          const uint32_t a1 = __byte_perm(x.v[0][w], x.v[1][w], 0x7362);
-          const uint32_t b0 = __byte_perm(x.v[2][w], x.v[3][w], 0x5140);
-          const uint32_t b1 = __byte_perm(x.v[2][w], x.v[3][w], 0x7362);
-          mma_f16(o[4 * w], pa, e4m3x2_to_f16x2(a0 & 0xffffu), e4m3x2_to_f16x2(b0 & 0xffffu));
-          mma_f16(o[4 * w + 1], pa, e4m3x2_to_f16x2(a0 >> 16), e4m3x2_to_f16x2(b0 >> 16));
-          mma_f16(o[4 * w + 2], pa, e4m3x2_to_f16x2(a1 & 0xffffu), e4m3x2_to_f16x2(b1 & 0xffffu));
-          mma_f16(o[4 * w + 3], pa, e4m3x2_to_f16x2(a1 >> 16), e4m3x2_to_f16x2(b1 >> 16));
-        } else {
-          mma_16816(o[2 * w], pa, __byte_perm(x.v[0][w], x.v[1][w], 0x5410),
-                    __byte_perm(x.v[2][w], x.v[3][w], 0x5410));
-          mma_16816(o[2 * w + 1], pa, __byte_perm(x.v[0][w], x.v[1][w], 0x7632),
-                    __byte_perm(x.v[2][w], x.v[3][w], 0x7632));
-        }
-      }
-    }
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
     }
 
     // Join the four warps, then the CTAs that share the job.
-    __syncthreads();
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int row = g + 8 * r;
-      if (row < rows_left) {
-        float* dst = sm_o + (warp * ROWS + row) * D;
+    for (int n = 0; n < NR; ++n)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          dst[2 * t4 * NT + nt] = o[nt][2 * r];
-          dst[(2 * t4 + 1) * NT + nt] = o[nt][2 * r + 1];
-        }
-        if (t4 == 0) {
-          sm_ml[(warp * ROWS + row) * 2] = m[r];
-          sm_ml[(warp * ROWS + row) * 2 + 1] = l[r];
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int o = 4; o <= 16; o <<= 1)
+          w.l[n][e] += __shfl_xor_sync(0xffffffffu, w.l[n][e], o);
+        const int row = 8 * n + 2 * t4 + e;
+        if (row < rows_left) {
+          float* dst = sm_o + (warp * ROWS + row) * LD + g * NT;
+#pragma unroll
+          for (int i = 0; i < NT / 2; i += 2)
+            *reinterpret_cast<float4*>(dst + 2 * i) =
+                make_float4(w.o[n][i][e], w.o[n][i][2 + e], w.o[n][i + 1][e], w.o[n][i + 1][2 + e]);
+          if (g == 0) {
+            sm_ml[(warp * ROWS + row) * 2] = w.m[n][e];
+            sm_ml[(warp * ROWS + row) * 2 + 1] = w.l[n][e];
+          }
         }
       }
-    }
     __syncthreads();
     const int64_t js = pre[b] + (int64_t)job * s.nb;
     const int64_t c0 = js / piece, c1 = (js + s.nb - 1) / piece;
     const int rows = min(ROWS, rows_left);
     const bool whole = c0 == c1;
     float* part = a.part + ((int64_t)blockIdx.x * 2 + (blockIdx.x == c0 ? 1 : 0)) * ROWS * (D + 2);
-    for (int idx = tid; idx < rows * D; idx += 128) {
-      const int row = idx / D, d = idx % D;
+    for (int i = tid; i < rows * D; i += 128) {
+      const int row = i / D, d = i % D;
       float M = kNegBig;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) M = fmaxf(M, sm_ml[(w * ROWS + row) * 2]);
+      for (int k = 0; k < 4; ++k) M = fmaxf(M, sm_ml[(k * ROWS + row) * 2]);
       float L = 0.f, O = 0.f;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const float f = exp2f(sm_ml[(w * ROWS + row) * 2] - M);
-        L += sm_ml[(w * ROWS + row) * 2 + 1] * f;
-        O += sm_o[(w * ROWS + row) * D + d] * f;
+      for (int k = 0; k < 4; ++k) {
+        const float f = ex2(sm_ml[(k * ROWS + row) * 2] - M);
+        L += sm_ml[(k * ROWS + row) * 2 + 1] * f;
+        O += sm_o[(k * ROWS + row) * LD + d] * f;
       }
       if (whole) {
         const int rr = tile * ROWS + row;
@@ -520,15 +583,15 @@ __global__ void __launch_bounds__(128) attn_rows_kernel(const Args a) {
       __syncthreads();
       if (s_last) {
         __threadfence();
-        for (int idx = tid; idx < rows * D; idx += 128) {
-          const int row = idx / D, d = idx % D;
+        for (int i = tid; i < rows * D; i += 128) {
+          const int row = i / D, d = i % D;
           float M = kNegBig, L = 0.f, O = 0.f;
           for (int64_t c = c0; c <= c1; ++c) {
             const float* src =
                 a.part + (c * 2 + (c == c0 ? 1 : 0)) * ROWS * (D + 2) + row * (D + 2);
             const float m_c = __ldcg(src), l_c = __ldcg(src + 1), o_c = __ldcg(src + 2 + d);
             const float m_new = fmaxf(M, m_c);
-            const float f0 = exp2f(M - m_new), f1 = exp2f(m_c - m_new);
+            const float f0 = ex2(M - m_new), f1 = ex2(m_c - m_new);
             L = L * f0 + l_c * f1;
             O = O * f0 + o_c * f1;
             M = m_new;
@@ -544,23 +607,30 @@ __global__ void __launch_bounds__(128) attn_rows_kernel(const Args a) {
   }
 }
 
-template <int D, bool FP8>
+template <int D, bool FP8, int NR>
 void launch_rows(const Args& a, int grid, cudaStream_t stream) {
-  const int smem = (a.B + 2) / 2 * 2 * 8 + 4 * 16 * (D + 2) * 4;
+  const int smem = (a.B + 2) / 2 * 2 * 8 + 4 * 8 * NR * (D + 6) * 4;
   static int configured = 0;
   if (smem > configured) {
-    CB_CUDA_CHECK(cudaFuncSetAttribute(attn_rows_kernel<D, FP8>,
+    CB_CUDA_CHECK(cudaFuncSetAttribute(attn_rows_kernel<D, FP8, NR>,
                                        cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     configured = smem;
   }
-  launch_kernel(attn_rows_kernel<D, FP8>, dim3(grid), dim3(128), smem, stream, a);
+  launch_kernel(attn_rows_kernel<D, FP8, NR>, dim3(grid), dim3(128), smem, stream, a);
+}
+
+// Query rows of a kv head and sequence up to 8: one column tile.
+template <int D, bool FP8>
+void launch(const Args& a, int64_t max_rows, cudaStream_t stream) {
+  if (max_rows <= 8) launch_rows<D, FP8, 1>(a, (FP8 ? 3 : 2) * num_sms(), stream);
+  else launch_rows<D, FP8, 2>(a, 2 * num_sms(), stream);
 }
 
 }  // namespace tree
 
-// {grid, workspace floats, workspace counters} of attn_tree.
+// {largest grid, workspace floats, workspace counters} of attn_tree.
 std::vector<int64_t> attn_tree_plan(int64_t head_dim) {
-  const int64_t grid = 2 * num_sms();
+  const int64_t grid = 3 * num_sms();
   return {grid, grid * 2 * 16 * (head_dim + 2), grid};
 }
 
@@ -641,13 +711,13 @@ void attn_tree(torch::Tensor q, torch::Tensor k_cache, torch::Tensor v_cache,
   a.G = (int)(q.size(1) / D / Hkv);
   a.scale_log2 = (float)scale * tree::kLog2e;
   cudaStream_t stream = at::cuda::getCurrentCUDAStream();
-  const int grid = (int)plan[0];
+  const int64_t rows = max_nodes * a.G;
   if (D == 128) {
-    if (fp8) tree::launch_rows<128, true>(a, grid, stream);
-    else tree::launch_rows<128, false>(a, grid, stream);
+    if (fp8) tree::launch<128, true>(a, rows, stream);
+    else tree::launch<128, false>(a, rows, stream);
   } else {
-    if (fp8) tree::launch_rows<64, true>(a, grid, stream);
-    else tree::launch_rows<64, false>(a, grid, stream);
+    if (fp8) tree::launch<64, true>(a, rows, stream);
+    else tree::launch<64, false>(a, rows, stream);
   }
 }
 
