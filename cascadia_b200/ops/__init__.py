@@ -305,7 +305,7 @@ def attn_tree(q, k_cache, v_cache, block_tables, seq_lens, row_start, out, layer
     plan = e.attn_tree_plan(k_cache.shape[4])
     ws.ensure(plan[1], plan[2])
     e.attn_tree(q, k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, row_start, masks,
-                out, layer, scale, max_nodes, ws.ws, ws.counters)
+                out, layer, scale, max_nodes, ws.ws, ws.counters, status_buffer(q.device))
     LAUNCHES.add(1)
     return out
 

@@ -24,43 +24,18 @@
 // on the device: a captured graph stays right when they change.  A job cut by
 // piece ends is joined by the last CTA that finishes a part of it, in the order
 // of the parts (the result does not depend on which CTA that is).
-#include <torch/extension.h>
+#include <ATen/core/Tensor.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <cuda_fp8.h>
 
+#include "attn_tree.cuh"
 #include "common.cuh"
 #include "host_utils.h"
 #include "mma_frag.cuh"
 
 namespace cb {
 namespace tree {
-
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kNegBig = -1e30f;
-constexpr int kMaxBatch = 4096;
-
-struct Args {
-  const __nv_bfloat16* q;
-  int64_t q_stride;
-  const uint8_t* k;
-  const uint8_t* v;
-  const float* ks;
-  const float* vs;
-  const int* table;
-  int64_t table_stride;
-  int table_width;
-  const int* seq_lens;
-  const int* row_start;
-  const int64_t* masks;
-  __nv_bfloat16* out;
-  int64_t out_stride;
-  float* part;    // [grid][2][rows][D + 2]
-  int* counters;  // [grid], zero between launches
-  int64_t layer_blocks;
-  int B, Hkv, G;
-  float scale_log2;
-};
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
                                         uint32_t b1) {
@@ -71,85 +46,11 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], u
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t pair) {
-  const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)pair, __NV_E4M3);
-  return (uint32_t)r.x | ((uint32_t)r.y << 16);
-}
-
-__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
-  const __half2 v = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&v);
-}
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 // Transpose of an 8 x 8 matrix of 16-bit values held two to a lane.
 __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
   uint32_t r;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
-}
-
-// Streaming load: a cache row is read once by one SM.
-__device__ __forceinline__ uint4 ldg_stream16(const void* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
-  return v;
-}
-__device__ __forceinline__ uint2 ldg_stream8(const void* p) {
-  uint2 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];"
-               : "=r"(v.x), "=r"(v.y)
-               : "l"(p));
-  return v;
-}
-
-struct SeqShape {
-  int n, len, nb, tiles;
-};
-
-__device__ __forceinline__ SeqShape seq_shape(const Args& a, int b, int rows) {
-  SeqShape s;
-  s.n = max(0, a.row_start[b + 1] - a.row_start[b]);
-  s.len = min(max(0, a.seq_lens[b]), a.table_width * 16);
-  s.nb = max(1, (s.len + 15) >> 4);
-  s.tiles = (s.n * a.G + rows - 1) / rows;
-  return s;
-}
-
-// pre[b] = 16-token blocks of work before sequence b; pre[B] = all of it.
-__device__ __forceinline__ void scan_work(const Args& a, int rows, int64_t* pre, int64_t* warp_sum) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  int64_t carry = 0;
-  if (tid == 0) pre[0] = 0;
-  for (int base = 0; base < a.B; base += 128) {
-    const int b = base + tid;
-    int64_t u = 0;
-    if (b < a.B) {
-      const SeqShape s = seq_shape(a, b, rows);
-      u = (int64_t)a.Hkv * s.tiles * s.nb;
-    }
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t x = __shfl_up_sync(0xffffffffu, u, o);
-      if (lane >= o) u += x;
-    }
-    if (lane == 31) warp_sum[warp] = u;
-    __syncthreads();
-    int64_t before = carry;
-    for (int w = 0; w < 4; ++w) {
-      if (w < warp) before += warp_sum[w];
-      carry += warp_sum[w];
-    }
-    if (b < a.B) pre[b + 1] = before + u;
-    __syncthreads();
-  }
 }
 
 // One warp's view of one 16-token block: K and V as loaded, and the scales.
@@ -416,7 +317,7 @@ __global__ void __launch_bounds__(128, NR == 1 && FP8 ? 3 : 2) attn_rows_kernel(
   grid_dep_launch();
   grid_dep_wait();
 
-  scan_work(a, ROWS, pre, s_sum);
+  scan_work<16, 128>(a, ROWS, pre, s_sum);
   const int64_t total = pre[a.B];
   // At least 8 blocks a piece: two for each warp.
   const int64_t piece = max((int64_t)8, (total + gridDim.x - 1) / gridDim.x);
@@ -424,16 +325,8 @@ __global__ void __launch_bounds__(128, NR == 1 && FP8 ? 3 : 2) attn_rows_kernel(
   const int64_t u_end = min(total, u + piece);
 
   while (u < u_end) {
-    int lo = 0, hi = a.B;  // pre[lo] <= u < pre[hi]
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (pre[mid] <= u) lo = mid;
-      else hi = mid;
-    }
-    // Sequences without rows share their successor's offset: the search ends
-    // on the last of them, the one with the work.
-    const int b = lo;
-    const SeqShape s = seq_shape(a, b, ROWS);
+    const int b = find_seq(pre, a.B, u);
+    const SeqShape s = seq_shape<16>(a, b, ROWS);
     const int64_t local = u - pre[b];
     const int job = (int)(local / s.nb);
     const int k0 = (int)(local - (int64_t)job * s.nb);
@@ -619,27 +512,29 @@ void launch_rows(const Args& a, int grid, cudaStream_t stream) {
   launch_kernel(attn_rows_kernel<D, FP8, NR>, dim3(grid), dim3(128), smem, stream, a);
 }
 
-// Query rows of a kv head and sequence up to 8: one column tile.
+// By the query rows of a kv head and sequence.
 template <int D, bool FP8>
 void launch(const Args& a, int64_t max_rows, cudaStream_t stream) {
   if (max_rows <= 8) launch_rows<D, FP8, 1>(a, (FP8 ? 3 : 2) * num_sms(), stream);
-  else launch_rows<D, FP8, 2>(a, 2 * num_sms(), stream);
+  else if (max_rows <= 16) launch_rows<D, FP8, 2>(a, 2 * num_sms(), stream);
+  else launch_tiles<D, FP8>(a, stream);
 }
 
 }  // namespace tree
 
 // {largest grid, workspace floats, workspace counters} of attn_tree.
 std::vector<int64_t> attn_tree_plan(int64_t head_dim) {
-  const int64_t grid = 3 * num_sms();
-  return {grid, grid * 2 * 16 * (head_dim + 2), grid};
+  const int64_t sms = num_sms();
+  return {3 * sms, sms * 2 * 256 * (head_dim + 2), 3 * sms};
 }
 
 // q, out: [rows, Hq * D]; rows of sequence b are row_start[b] .. row_start[b+1].
-void attn_tree(torch::Tensor q, torch::Tensor k_cache, torch::Tensor v_cache,
-               c10::optional<torch::Tensor> k_scale, c10::optional<torch::Tensor> v_scale,
-               torch::Tensor block_tables, torch::Tensor seq_lens, torch::Tensor row_start,
-               c10::optional<torch::Tensor> masks, torch::Tensor out, int64_t layer, double scale,
-               int64_t max_nodes, torch::Tensor ws, torch::Tensor counters) {
+void attn_tree(at::Tensor q, at::Tensor k_cache, at::Tensor v_cache,
+               c10::optional<at::Tensor> k_scale, c10::optional<at::Tensor> v_scale,
+               at::Tensor block_tables, at::Tensor seq_lens, at::Tensor row_start,
+               c10::optional<at::Tensor> masks, at::Tensor out, int64_t layer, double scale,
+               int64_t max_nodes, at::Tensor ws, at::Tensor counters,
+               at::Tensor status) {
   TORCH_CHECK(q.is_cuda() && q.dim() == 2 && q.scalar_type() == at::kBFloat16 &&
                   out.dim() == 2 && out.scalar_type() == at::kBFloat16 && q.stride(1) == 1 &&
                   out.stride(1) == 1 && out.size(0) >= q.size(0) && out.size(1) == q.size(1),
@@ -658,18 +553,18 @@ void attn_tree(torch::Tensor q, torch::Tensor k_cache, torch::Tensor v_cache,
   TORCH_CHECK(q.size(1) % D == 0 && (q.size(1) / D) % Hkv == 0, "query heads must divide");
   TORCH_CHECK(layer >= 0 && layer < k_cache.size(0), "layer outside the cache");
   const int64_t B = seq_lens.numel();
-  TORCH_CHECK(B <= tree::kMaxBatch, "at most 4096 sequences");
+  TORCH_CHECK(B <= tree::kMaxBatch, "at most 2048 sequences");
   TORCH_CHECK(block_tables.scalar_type() == at::kInt && block_tables.dim() == 2 &&
                   block_tables.size(0) >= B && block_tables.stride(1) == 1 &&
                   seq_lens.scalar_type() == at::kInt && seq_lens.is_contiguous() &&
                   row_start.scalar_type() == at::kInt && row_start.is_contiguous() &&
                   row_start.numel() >= B + 1,
               "int32 block tables [B, W], seq lens [B] and row starts [B + 1]");
-  for (const torch::Tensor* t :
+  for (const at::Tensor* t :
        {&out, &k_cache, &v_cache, &block_tables, &seq_lens, &row_start, &ws, &counters})
     TORCH_CHECK(t->device() == q.device(), "all tensors must be on one device");
   if (fp8) {
-    for (const torch::Tensor* t : {&*k_scale, &*v_scale})
+    for (const at::Tensor* t : {&*k_scale, &*v_scale})
       TORCH_CHECK(t->scalar_type() == at::kFloat && t->is_contiguous() &&
                       t->numel() == k_cache.numel() / D && t->device() == q.device(),
                   "k/v scales must be fp32 [L, NB, Hkv, 16] contiguous");
@@ -705,6 +600,8 @@ void attn_tree(torch::Tensor q, torch::Tensor k_cache, torch::Tensor v_cache,
   a.out_stride = out.stride(0);
   a.part = ws.data_ptr<float>();
   a.counters = counters.data_ptr<int>();
+  a.status = status.data_ptr<int>();
+  a.out_vec = (out.stride(0) * 2) % 16 == 0 && reinterpret_cast<uintptr_t>(out.data_ptr()) % 16 == 0;
   a.layer_blocks = layer * k_cache.size(1);
   a.B = (int)B;
   a.Hkv = Hkv;

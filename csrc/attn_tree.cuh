@@ -1,0 +1,139 @@
+// What the attention kernels over new tokens share: arguments, the split of the
+// work, and small device helpers.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "common.cuh"
+
+namespace cb {
+namespace tree {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kNegBig = -1e30f;
+constexpr int kMaxBatch = 2048;
+
+struct Args {
+  const __nv_bfloat16* q;
+  int64_t q_stride;
+  const uint8_t* k;
+  const uint8_t* v;
+  const float* ks;
+  const float* vs;
+  const int* table;
+  int64_t table_stride;
+  int table_width;
+  const int* seq_lens;
+  const int* row_start;
+  const int64_t* masks;
+  __nv_bfloat16* out;
+  int64_t out_stride;
+  float* part;    // two partial results for each CTA
+  int* counters;  // [grid], zero between launches
+  int* status;
+  int64_t layer_blocks;
+  int B, Hkv, G;
+  int out_vec;  // output rows are 16-byte aligned
+  float scale_log2;
+};
+
+__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t pair) {
+  const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)pair, __NV_E4M3);
+  return (uint32_t)r.x | ((uint32_t)r.y << 16);
+}
+
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Streaming load: a cache row is read once by one SM.
+__device__ __forceinline__ uint4 ldg_stream16(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint2 ldg_stream8(const void* p) {
+  uint2 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];"
+               : "=r"(v.x), "=r"(v.y)
+               : "l"(p));
+  return v;
+}
+
+// n rows, len keys in nb units of UNIT tokens (one at least), read by `tiles`
+// row tiles.
+struct SeqShape {
+  int n, len, nb, tiles;
+};
+
+template <int UNIT>
+__device__ __forceinline__ SeqShape seq_shape(const Args& a, int b, int rows) {
+  SeqShape s;
+  s.n = max(0, a.row_start[b + 1] - a.row_start[b]);
+  s.len = min(max(0, a.seq_lens[b]), a.table_width * 16);
+  s.nb = max(1, (s.len + UNIT - 1) / UNIT);
+  s.tiles = (s.n * a.G + rows - 1) / rows;
+  return s;
+}
+
+// pre[b] = units of work before sequence b; pre[B] = all of it.
+template <int UNIT, int THREADS>
+__device__ __forceinline__ void scan_work(const Args& a, int rows, int64_t* pre, int64_t* warp_sum) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int64_t carry = 0;
+  if (tid == 0) pre[0] = 0;
+  for (int base = 0; base < a.B; base += THREADS) {
+    const int b = base + tid;
+    int64_t u = 0;
+    if (b < a.B) {
+      const SeqShape s = seq_shape<UNIT>(a, b, rows);
+      u = (int64_t)a.Hkv * s.tiles * s.nb;
+    }
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t x = __shfl_up_sync(0xffffffffu, u, o);
+      if (lane >= o) u += x;
+    }
+    if (lane == 31) warp_sum[warp] = u;
+    __syncthreads();
+    int64_t before = carry;
+    for (int w = 0; w < THREADS / 32; ++w) {
+      if (w < warp) before += warp_sum[w];
+      carry += warp_sum[w];
+    }
+    if (b < a.B) pre[b + 1] = before + u;
+    __syncthreads();
+  }
+}
+
+// The sequence that unit u belongs to: pre[b] <= u < pre[b + 1].  Sequences
+// without rows share their successor's offset: the search ends on the last of
+// them, the one with the work.
+__device__ __forceinline__ int find_seq(const int64_t* pre, int B, int64_t u) {
+  int lo = 0, hi = B;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (pre[mid] <= u) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// Rows of a kv head and sequence above this run on the tile kernel.
+template <int D, bool FP8>
+void launch_tiles(const Args& a, cudaStream_t stream);
+
+}  // namespace tree
+}  // namespace cb

@@ -129,7 +129,8 @@ void attn_tree(torch::Tensor q, torch::Tensor k_cache, torch::Tensor v_cache,
                c10::optional<torch::Tensor> k_scale, c10::optional<torch::Tensor> v_scale,
                torch::Tensor block_tables, torch::Tensor seq_lens, torch::Tensor row_start,
                c10::optional<torch::Tensor> masks, torch::Tensor out, int64_t layer, double scale,
-               int64_t max_nodes, torch::Tensor ws, torch::Tensor counters);
+               int64_t max_nodes, torch::Tensor ws, torch::Tensor counters,
+               torch::Tensor status);
 // logprobs.cu
 std::vector<int64_t> token_logprobs_plan(int64_t rows, int64_t vocab, int64_t elem_size);
 void token_logprobs(torch::Tensor logits, torch::Tensor tokens, int64_t top_k,

@@ -10,7 +10,7 @@
 // log2 s finite for a row of zeros.  A row that holds a NaN or an infinity gets
 // s = NaN and zero codes: it reads back as NaN, and an attention row that does
 // not see it never multiplies by it.
-#include <torch/extension.h>
+#include <ATen/core/Tensor.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <cuda_fp8.h>
@@ -246,8 +246,8 @@ __global__ void __launch_bounds__(256) kv_read_fp8_kernel(const ReadArgs a) {
 
 // ---------------------------------------------------------------- host side
 
-static void check_fp8_cache(const torch::Tensor& k, const torch::Tensor& v,
-                            const torch::Tensor& ks, const torch::Tensor& vs) {
+static void check_fp8_cache(const at::Tensor& k, const at::Tensor& v,
+                            const at::Tensor& ks, const at::Tensor& vs) {
   TORCH_CHECK(k.is_cuda() && k.scalar_type() == at::kFloat8_e4m3fn &&
                   v.scalar_type() == at::kFloat8_e4m3fn,
               "k/v cache must be float8_e4m3fn on the GPU");
@@ -278,11 +278,11 @@ static void launch_write(const WriteArgs& a, cudaStream_t stream) {
   }
 }
 
-void rope_kv_write_fp8(torch::Tensor qkv, torch::Tensor positions, torch::Tensor cos_sin,
-                       torch::Tensor slots, torch::Tensor k_cache, torch::Tensor v_cache,
-                       torch::Tensor k_scale, torch::Tensor v_scale, int64_t layer, int64_t Hq,
+void rope_kv_write_fp8(at::Tensor qkv, at::Tensor positions, at::Tensor cos_sin,
+                       at::Tensor slots, at::Tensor k_cache, at::Tensor v_cache,
+                       at::Tensor k_scale, at::Tensor v_scale, int64_t layer, int64_t Hq,
                        int64_t Hkv, int64_t D, int64_t rot, bool interleaved,
-                       c10::optional<torch::Tensor> q_out) {
+                       c10::optional<at::Tensor> q_out) {
   check_fp8_cache(k_cache, v_cache, k_scale, v_scale);
   TORCH_CHECK(qkv.dim() == 2 && qkv.scalar_type() == at::kBFloat16 && qkv.stride(1) == 1 &&
                   qkv.size(1) == (Hq + 2 * Hkv) * D,
@@ -299,7 +299,7 @@ void rope_kv_write_fp8(torch::Tensor qkv, torch::Tensor positions, torch::Tensor
   TORCH_CHECK(cos_sin.scalar_type() == at::kFloat && cos_sin.is_contiguous() &&
                   cos_sin.dim() == 2 && cos_sin.size(1) == rot,
               "cos_sin must be fp32 [positions, rot]");
-  torch::Tensor qo = q_out.has_value() ? *q_out : qkv;
+  at::Tensor qo = q_out.has_value() ? *q_out : qkv;
   TORCH_CHECK(qo.scalar_type() == at::kBFloat16 && qo.dim() == 2 && qo.stride(1) == 1 &&
                   qo.size(0) >= T && qo.size(1) >= Hq * D,
               "q_out must be bf16 [T, Hq D] with inner stride 1");
@@ -338,16 +338,16 @@ void rope_kv_write_fp8(torch::Tensor qkv, torch::Tensor positions, torch::Tensor
   else launch_write<256>(a, stream);
 }
 
-void kv_read_fp8(torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor k_scale,
-                 torch::Tensor v_scale, torch::Tensor blocks, int64_t layer, torch::Tensor k_out,
-                 torch::Tensor v_out) {
+void kv_read_fp8(at::Tensor k_cache, at::Tensor v_cache, at::Tensor k_scale,
+                 at::Tensor v_scale, at::Tensor blocks, int64_t layer, at::Tensor k_out,
+                 at::Tensor v_out) {
   check_fp8_cache(k_cache, v_cache, k_scale, v_scale);
   const int64_t N = blocks.numel(), Hkv = k_cache.size(2), D = k_cache.size(4);
   TORCH_CHECK(D == 64 || D == 128 || D == 256, "head_dim must be 64, 128 or 256");
   TORCH_CHECK(layer >= 0 && layer < k_cache.size(0), "layer outside the cache");
   TORCH_CHECK(blocks.scalar_type() == at::kInt && blocks.is_contiguous(),
               "blocks must be contiguous int32");
-  for (const torch::Tensor* o : {&k_out, &v_out}) {
+  for (const at::Tensor* o : {&k_out, &v_out}) {
     TORCH_CHECK(o->scalar_type() == at::kBFloat16 && o->is_contiguous() &&
                     o->numel() >= N * Hkv * 16 * D &&
                     reinterpret_cast<uintptr_t>(o->data_ptr()) % 16 == 0,

@@ -19,7 +19,7 @@
 //
 // A row is cut in slices, one for each CTA, when there are few rows; the last
 // CTA of a row joins them.
-#include <torch/extension.h>
+#include <ATen/core/Tensor.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
@@ -425,9 +425,9 @@ std::vector<int64_t> token_logprobs_plan(int64_t rows, int64_t vocab, int64_t el
   return {s, s > 1 ? rows * s * (4 + 2 * lp::kMaxTop) : 0, s > 1 ? rows : 0};
 }
 
-void token_logprobs(torch::Tensor logits, torch::Tensor tokens, int64_t top_k,
-                    torch::Tensor logprob, torch::Tensor entropy, torch::Tensor top_ids,
-                    torch::Tensor top_lp, torch::Tensor ws, torch::Tensor counters) {
+void token_logprobs(at::Tensor logits, at::Tensor tokens, int64_t top_k,
+                    at::Tensor logprob, at::Tensor entropy, at::Tensor top_ids,
+                    at::Tensor top_lp, at::Tensor ws, at::Tensor counters) {
   TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && logits.stride(1) == 1 && logits.size(1) > 0,
               "logits must be [rows, vocab] with inner stride 1");
   const auto type = logits.scalar_type();

@@ -34,6 +34,7 @@ SOURCES = [
     "ffn_sparse.cu",
     "kv_fp8.cu",
     "attn_tree.cu",
+    "attn_tree_tiles.cu",
     "logprobs.cu",
 ]
 
