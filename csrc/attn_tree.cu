@@ -15,7 +15,8 @@
 // so that the weights of the value codes stay in [0, 1] whatever the scales
 // are, for one exponential a score.  e4m3 codes are exact in fp16; q is brought
 // into fp16's range by a power of two of its own for every row, and the weights
-// are held as 2^15 w in fp16 (11 bits).  With the bf16 cache the weights are
+// are held as 2^8 w in fp16 (11 bits; w / vs summed over 2^19 keys stays finite
+// down to the smallest scale, 2^-100).  With the bf16 cache the weights are
 // rounded to bf16, as its values are.  Sums and statistics are fp32.
 //
 // Work split: the keys of all (sequence, kv head, row tile) jobs form one line
@@ -24,6 +25,9 @@
 // on the device: a captured graph stays right when they change.  A job cut by
 // piece ends is joined by the last CTA that finishes a part of it, in the order
 // of the parts (the result does not depend on which CTA that is).
+//
+// Up to 16 query rows of a kv head and sequence run here, on warp-level products
+// fed from registers; more run on the tile kernel (attn_tree_tiles.cu).
 #include <ATen/core/Tensor.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -32,7 +36,6 @@
 #include "attn_tree.cuh"
 #include "common.cuh"
 #include "host_utils.h"
-#include "mma_frag.cuh"
 
 namespace cb {
 namespace tree {
@@ -45,6 +48,8 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], u
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+
+constexpr float kUp = 8.f;  // fp16 weights are held as 2^kUp w
 
 // Transpose of an 8 x 8 matrix of 16-bit values held two to a lane.
 __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
@@ -135,8 +140,9 @@ struct Warp {
       if constexpr (FP8) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const uint32_t kf[4] = {e4m3x2_to_f16x2(w0[i] & 0xffffu), e4m3x2_to_f16x2(w1[i] & 0xffffu),
-                                  e4m3x2_to_f16x2(w0[i] >> 16), e4m3x2_to_f16x2(w1[i] >> 16)};
+          uint32_t kf[4];
+          e4m3_to_f16(w0[i], kf[0], kf[2]);
+          e4m3_to_f16(w1[i], kf[1], kf[3]);
 #pragma unroll
           for (int n = 0; n < NR; ++n) mma_f16(sc[n], kf, q[n][4 * c + i][0], q[n][4 * c + i][1]);
         }
@@ -203,7 +209,7 @@ struct Warp {
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
         const float m_new = fmaxf(m[n][e], mx);
         alpha[e] = ex2(m[n][e] - m_new);
-        const float base = FP8 ? m_new - 15.f : m_new;
+        const float base = FP8 ? m_new - kUp : m_new;
         m[n][e] = m_new;
         float sum = 0.f;
 #pragma unroll
@@ -235,15 +241,12 @@ struct Warp {
 #pragma unroll
     for (int w = 0; w < Block<D, FP8>::VW; ++w) {
       if constexpr (FP8) {
-        // Bytes of two tokens side by side, four dims a word.
-        const uint32_t a0 = __byte_perm(x.v[0][w], x.v[1][w], 0x5140);
-        const uint32_t a1 = __byte_perm(x.v[0][w], x.v[1][w], 0x7362);
-        const uint32_t b0 = __byte_perm(x.v[2][w], x.v[3][w], 0x5140);
-        const uint32_t b1 = __byte_perm(x.v[2][w], x.v[3][w], 0x7362);
-        const uint32_t v0[4] = {e4m3x2_to_f16x2(a0 & 0xffffu), e4m3x2_to_f16x2(a0 >> 16),
-                                e4m3x2_to_f16x2(b0 & 0xffffu), e4m3x2_to_f16x2(b0 >> 16)};
-        const uint32_t v1[4] = {e4m3x2_to_f16x2(a1 & 0xffffu), e4m3x2_to_f16x2(a1 >> 16),
-                                e4m3x2_to_f16x2(b1 & 0xffffu), e4m3x2_to_f16x2(b1 >> 16)};
+        // Bytes of two tokens side by side, two dims a word.
+        uint32_t v0[4], v1[4];
+        e4m3_to_f16(__byte_perm(x.v[0][w], x.v[1][w], 0x5410), v0[0], v0[1]);
+        e4m3_to_f16(__byte_perm(x.v[2][w], x.v[3][w], 0x5410), v0[2], v0[3]);
+        e4m3_to_f16(__byte_perm(x.v[0][w], x.v[1][w], 0x7632), v1[0], v1[1]);
+        e4m3_to_f16(__byte_perm(x.v[2][w], x.v[3][w], 0x7632), v1[2], v1[3]);
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
           mma_f16(o[n][2 * w], v0, pf[n][0], pf[n][1]);
@@ -375,15 +378,15 @@ __global__ void __launch_bounds__(128, NR == 1 && FP8 ? 3 : 2) attn_rows_kernel(
         const int e = (int)(top >> 7);  // biased exponent
         const int sh = e == 0 || e == 255 ? 0 : min(100, 127 + 14 - e);
         const float up = __int_as_float((127 + sh) << 23);
-        back *= __int_as_float((127 - sh) << 23);
+        back *= __int_as_float((127 + 8 - sh) << 23);  // (keys are unpacked times 2^-8)
+        // Dims 0, 2 and 1, 3 of every four, as the keys' codes are unpacked.
 #pragma unroll
-        for (int ks = 0; ks < NKS; ++ks)
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const uint32_t y = w.q[n][ks][k];
-            w.q[n][ks][k] = pack_f16(__uint_as_float(y << 16) * up,
-                                     __uint_as_float(y & 0xffff0000u) * up);
-          }
+        for (int ks = 0; ks < NKS; ++ks) {
+          const uint32_t lo = w.q[n][ks][0], hi = w.q[n][ks][1];
+          w.q[n][ks][0] = pack_f16(__uint_as_float(lo << 16) * up, __uint_as_float(hi << 16) * up);
+          w.q[n][ks][1] = pack_f16(__uint_as_float(lo & 0xffff0000u) * up,
+                                   __uint_as_float(hi & 0xffff0000u) * up);
+        }
       }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
@@ -456,7 +459,7 @@ __global__ void __launch_bounds__(128, NR == 1 && FP8 ? 3 : 2) attn_rows_kernel(
       if (whole) {
         const int rr = tile * ROWS + row;
         a.out[(int64_t)(q_row0 + rr / a.G) * a.out_stride + (int64_t)(h * a.G + rr % a.G) * D + d] =
-            __float2bfloat16(L == 0.f ? 0.f : O / L);
+            __float2bfloat16(L == 0.f ? 0.f : (FP8 ? 256.f * O : O) / L);
       } else {
         part[row * (D + 2) + 2 + d] = O;
         if (d == 0) {
@@ -491,7 +494,7 @@ __global__ void __launch_bounds__(128, NR == 1 && FP8 ? 3 : 2) attn_rows_kernel(
           }
           const int rr = tile * ROWS + row;
           a.out[(int64_t)(q_row0 + rr / a.G) * a.out_stride + (int64_t)(h * a.G + rr % a.G) * D +
-                d] = __float2bfloat16(L == 0.f ? 0.f : O / L);
+                d] = __float2bfloat16(L == 0.f ? 0.f : (FP8 ? 256.f * O : O) / L);
         }
       }
     }

@@ -8,6 +8,7 @@
 #include <stdint.h>
 
 #include "common.cuh"
+#include "mma_frag.cuh"
 
 namespace cb {
 namespace tree {
@@ -40,9 +41,15 @@ struct Args {
   float scale_log2;
 };
 
-__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t pair) {
-  const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)pair, __NV_E4M3);
-  return (uint32_t)r.x | ((uint32_t)r.y << 16);
+// 4 e4m3 codes as fp16 times 2^-8, exact: the exponent and mantissa bits move
+// into place, the biases differ by 8 and e4m3's subnormals become fp16's.  even
+// holds codes 0 and 2 of the word, odd 1 and 3.  Seven integer instructions for
+// four codes; the conversion instruction runs on the unit that computes the
+// exponentials.  The code of a NaN does not come out as one; the writer never
+// stores it.
+__device__ __forceinline__ void e4m3_to_f16(uint32_t w, uint32_t& even, uint32_t& odd) {
+  even = ((w << 8) & 0x80008000u) | ((w << 7) & 0x3f803f80u);
+  odd = (w & 0x80008000u) | ((w >> 1) & 0x3f803f80u);
 }
 
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
@@ -59,14 +66,14 @@ __device__ __forceinline__ float ex2(float x) {
 // Streaming load: a cache row is read once by one SM.
 __device__ __forceinline__ uint4 ldg_stream16(const void* p) {
   uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+  asm("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
                : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
                : "l"(p));
   return v;
 }
 __device__ __forceinline__ uint2 ldg_stream8(const void* p) {
   uint2 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];"
+  asm("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];"
                : "=r"(v.x), "=r"(v.y)
                : "l"(p));
   return v;

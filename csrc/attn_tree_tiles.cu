@@ -1,25 +1,37 @@
 // Attention over the paged cache for many new tokens: 128 query rows of a kv
 // head a tile, on the tcgen05 tensor cores (formulas in attn_tree.cu).
 //
-// One CTA an SM, 13 warps:
+// One CTA an SM:
 //   warps 0-3, 4-7  softmax, one thread a row;
-//   warps 8-11      K / V: global memory -> registers -> (e4m3 to fp16) -> shared
-//                   memory in the 128-byte swizzle, two stages of 128 tokens;
-//   warp 12         one thread issues the products.
-// Tensor memory (512 columns): scores S0, S1 and sums O0, O1.  S = Q K^T reads
-// both operands from shared memory; the weights overwrite their scores as 16-bit
-// pairs and enter O += P V from there, V as it lies ([token][dim], dims contiguous).
+//   warps 8-15      K and V: global memory -> registers -> shared memory in the
+//                   128-byte swizzle, two stages of 128 tokens, 64 tokens for each
+//                   four warps;
+//   warps 16-19     one thread of each issues the products.
+// Tensor memory (512 columns): for each softmax group the scores of two steps of 64
+// tokens and the sums.  S = Q K^T reads both operands from shared memory; the weights
+// overwrite their scores as 16-bit pairs and enter O += P V from there, V as it lies
+// ([token][dim], dims contiguous).  While a group computes the weights of one step
+// the scores of its next are made: a step of 128 tokens with one score buffer left
+// every group idle for its products, twice the time.
 // With more than 128 rows a job has two row tiles, one for each softmax group,
 // that share every K / V tile; otherwise the groups take K / V tiles in turn and
-// their sums are joined at the end.  Either way one group's products run while
-// the other computes its weights.
+// their sums are joined at the end.
 //
-// The sums are rescaled only when a row's maximum has grown by more than 2^8
-// since they were last (weights then stay below 2^8: fp16 weights are held as
-// 2^7 w, below 2^15).
-#include <ATen/core/Tensor.h>
-#include <cuda_fp8.h>
-
+// 8-bit cache.  Scores: the codes of K enter an 8-bit product as they are, q as two
+// e4m3 numbers (q = hi + lo to its last bit, down to 2^-9 of the row's largest value;
+// below that to 2^-18 of it), at twice the rate of a 16-bit product, so that no key
+// has to be unpacked; a score is then multiplied by its key's scale.  Values: code x
+// scale / r in fp16, with r a power of two, the largest scale of the 128-token tile
+// rounded up, so that a softmax thread needs one number a tile for them instead of
+// two for each column (shared-memory bandwidth).  The price is one rounding to
+// fp16's 11 bits, 2^-12 of a value against the 2^-5 of its code and the 2^-9 of the
+// bf16 result; the scale itself enters as a pair of fp16 numbers, 22 bits.
+//
+// Weights are computed in one pass over the scores, in the frame of the maximum
+// that the row had before; only if a score is more than 2^8 over it (or keys of
+// the tile are hidden) the tile is taken again in two passes and the sums are
+// rescaled.  Weights thus stay below 2^8: fp16 weights are held as 2^7 w, below
+// 2^15.
 #include "attn_tree.cuh"
 #include "common.cuh"
 #include "host_utils.h"
@@ -28,18 +40,31 @@ namespace cb {
 namespace tree {
 
 constexpr int kTok = 128;          // tokens of a K / V tile
+constexpr int kStep = 64;           // tokens of a step
+constexpr int kSb = 128 / kStep;    // score buffers of a softmax group
+constexpr int kSpt = kTok / kStep;  // steps of a tile
 constexpr int kTileRows = 256;     // query rows of a job: two tiles of 128
-constexpr int kTileThreads = 416;  // 13 warps
-constexpr int kScaleBufs = 4;
+constexpr int kTileThreads = 640;
+// Registers of a thread: at launch, and after the groups have shared them out.
+constexpr int kRegsLaunch = 96, kRegsSoftmax = 128, kRegsLoad = 88, kRegsIssue = 48;
+static_assert(2 * kRegsSoftmax + 2 * kRegsLoad + kRegsIssue <= 5 * kRegsLaunch,
+              "more registers than the block has: the groups would wait for them for ever");
+static_assert(kRegsLoad <= kRegsLaunch && kRegsIssue <= kRegsLaunch && kRegsLaunch <= kRegsSoftmax,
+              "a share may only shrink below the launch's, or grow above it");
+constexpr int kTileBufs = 8;       // tiles whose scale references are kept
 
-template <int D>
+template <int D, bool FP8>
 struct TileSmem {
-  static constexpr int kOperand = 128 * D * 2;     // one K, V or Q tile
-  static constexpr int kK = 0;                     // [2]
-  static constexpr int kV = 2 * kOperand;          // [2]
-  static constexpr int kQ = 4 * kOperand;          // [2]
-  static constexpr int kScales = 6 * kOperand;     // [kScaleBufs][3][128] fp32
-  static constexpr int kMl = kScales + kScaleBufs * 3 * kTok * 4;  // [2][128][2]
+  static constexpr int kSlab = 128 * 128;             // 128 rows of 128 bytes
+  static constexpr int kVTile = D / 64 * kSlab;       // 16-bit values
+  static constexpr int kKTile = FP8 ? kSlab : kVTile;  // codes: one slab, also half filled
+  static constexpr int kQTile = FP8 ? 2 * kSlab : kVTile;
+  static constexpr int kK = 0;                       // [2]
+  static constexpr int kV = kK + 2 * kKTile;         // [2]
+  static constexpr int kQ = kV + 2 * kVTile;         // [2]
+  static constexpr int kScale = kQ + 2 * kQTile;     // K's: [kTileBufs][128] fp32
+  static constexpr int kPairs = kScale + kTileBufs * kTok * 4;  // V's: [8 warps][128]
+  static constexpr int kMl = kPairs + 8 * kTok * 4;  // [2][128][2]
   static constexpr int kBars = kMl + 2 * 128 * 2 * 4;
   static constexpr int kPre = kBars + 256;
   static int bytes(int B) { return kPre + (B + 2) / 2 * 2 * 8 + 1024; }
@@ -58,20 +83,28 @@ __device__ __forceinline__ uint64_t desc_v(uint32_t addr, uint32_t slab) {
   return d;
 }
 
-// 128 x n products of 16-bit values with fp32 sums.
-template <bool F16>
-__device__ constexpr uint32_t idesc(int n, bool b_mn_major) {
-  return (1u << 4) | (F16 ? 0u : (1u << 7) | (1u << 10)) | (b_mn_major ? 1u << 16 : 0u) |
+// 128 x n products with fp32 sums; format 0: fp16 (or e4m3, in an 8-bit product),
+// 1: bf16.
+__device__ constexpr uint32_t idesc(uint32_t format, int n, bool b_mn_major) {
+  return (1u << 4) | (format << 7) | (format << 10) | (b_mn_major ? 1u << 16 : 0u) |
          ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 }
 
-__device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&v)[32]) {
-  uint32_t r[32];
+// D[tmem] (+)= A[smem] * B[smem], e4m3 inputs (32 summed values), fp32 sums.
+__device__ __forceinline__ void mma_e4m3_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                            uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate));
+}
+
+__device__ __forceinline__ void tmem_ld32_start(uint32_t addr, uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
       "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
-      "tcgen05.wait::ld.sync.aligned;"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
         "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
         "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
@@ -79,8 +112,79 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&v)[32]) {
         "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(addr)
       : "memory");
-#pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+// The registers pass through the wait, so that nothing reads them before it.
+__device__ __forceinline__ void tmem_ld32_wait(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]),
+                 "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
+                 "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]),
+                 "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                 "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                 "+r"(r[30]), "+r"(r[31])::"memory");
+}
+
+__device__ __forceinline__ bool elect_one() {
+  uint32_t e;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(e));
+  return e != 0;
+}
+
+template <int N>
+__device__ __forceinline__ void more_registers() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void fewer_registers() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+// Two fp32 operations in one instruction.
+struct F2 {
+  uint64_t v;
+};
+__device__ __forceinline__ F2 f2(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void split(F2 x, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x.v));
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+
+__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
 }
 
 // Which of the 32 keys from position p0 on a row sees.
@@ -112,603 +216,809 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* s
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, status, kStatusAttnTimeout, abort_flag));
 }
 
+// Work is counted in 64 bits but hardly ever needs them.
+__device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
+  if (((a | b) >> 32) == 0) return (int64_t)((uint32_t)a / (uint32_t)b);
+  return a / b;
+}
+
+// One CTA's share of one job: K / V tiles k0 .. k0 + nt of (sequence b, kv head h,
+// row tile).
+struct Segment {
+  int b, h, n, len, ctx, nb, k0, nt, rows, mt;
+  int row0;      // first of the job's rows, node * G + head of the group
+  int q_row0;    // first query row of the sequence
+  const int* table;
+  int64_t c0, c1;  // CTAs that share the job
+  int64_t units;
+};
+
+// K / V tiles of softmax group w: all of them with two row tiles, every other one
+// with one.
+__device__ __forceinline__ int group_tiles(int nt, int mt, int w) {
+  return mt == 2 ? nt : (nt + 1 - w) >> 1;
+}
+
+__device__ __forceinline__ Segment segment_at(const Args& a, const int64_t* pre, int64_t u,
+                                              int64_t u_end, int64_t piece, bool skip) {
+  Segment g;
+  g.b = find_seq(pre, a.B, u);
+  const SeqShape s = seq_shape<kTok>(a, g.b, kTileRows);
+  const int64_t local = u - pre[g.b];
+  const int job = (int)divide(local, s.nb);
+  g.k0 = (int)(local - (int64_t)job * s.nb);
+  g.units = min((int64_t)s.nb - g.k0, u_end - u);
+  g.h = job / s.tiles;
+  g.row0 = (job - g.h * s.tiles) * kTileRows;
+  g.n = s.n;
+  g.len = s.len;
+  g.nb = s.nb;
+  g.ctx = s.len - s.n;
+  g.table = a.table + (int64_t)g.b * a.table_stride;
+  g.q_row0 = a.row_start[g.b];
+  g.rows = min(kTileRows, s.n * a.G - g.row0);
+  g.mt = g.rows > 128 ? 2 : 1;
+  g.nt = skip ? 0 : max(0, min(g.k0 + (int)g.units, (s.len + kTok - 1) / kTok) - g.k0);
+  const int64_t js = pre[g.b] + (int64_t)job * s.nb;
+  g.c0 = divide(js, piece);
+  g.c1 = divide(js + s.nb - 1, piece);
+  return g;
+}
+
+// What the loading groups share with the others.
+struct LoadSmem {
+  uint32_t k, v;      // [2] operand tiles (shared addresses)
+  uint32_t pairs;     // this warp's [128] scales of V over the reference, as fp16 pairs
+  float* k_scale;     // [kTileBufs][128]
+  float* v_ref;       // [kTileBufs]: log2 of V's reference / 2^6
+  uint64_t *k_full, *v_full, *k_free, *v_free;  // [2]
+  uint64_t* r_full;   // [kTileBufs]
+  volatile int* abort_flag;
+  int* nonfinite;
+};
+
+// Four warps bring 64 tokens of every K / V tile of the CTA's jobs into shared
+// memory.  As a row is stored, the same row of the next tile takes its registers,
+// so that half a tile's loads are always in flight for each group.
+template <int D, bool FP8>
+__device__ __forceinline__ void load_tiles(const Args& a, const int64_t* pre, int64_t u0,
+                                           int64_t u_end, int64_t piece, const LoadSmem& sm,
+                                           int group) {
+  using S = TileSmem<D, FP8>;
+  constexpr int RB = FP8 ? D : 2 * D;      // bytes of a cache row
+  constexpr int LPT = RB / 16;             // lanes that share a row, 16 bytes each
+  constexpr int TPW = 32 / LPT;            // rows of one warp-wide load
+  constexpr int ROWS = 64 / (4 * TPW);     // loads of a lane for its part of a tile
+  constexpr int NI = ROWS < 4 ? ROWS : 4;  // of them in flight, of K and of V
+  constexpr int PARTS = ROWS / NI;
+  const int ct = threadIdx.x & 127, cw = ct >> 5, lane = ct & 31;
+  // Lanes in fours along a row, then over two rows: the eight lanes of a store
+  // phase then write different banks, also when each writes every other chunk.
+  const int piece16 = LPT <= 4 ? lane % LPT : (lane & 3) | (lane >> 3 & (LPT / 4 - 1)) << 2;
+  const int sub = 64 * group + cw * TPW +
+                  (LPT <= 4 ? lane / LPT : (lane >> 2 & 1) | (lane >> 3) / (LPT / 4) << 1);
+  // Token of this lane's i-th row.
+  auto token_of = [&](int i) { return i * 4 * TPW + sub; };
+  // Its 16-byte chunk of a tile row: of K, and of V (8-bit: the first of two).
+  const int k_chunk = piece16 & 7, v_chunk = FP8 ? (2 * piece16) & 7 : piece16 & 7;
+  const uint32_t k_tiles = sm.k + (piece16 >> 3) * S::kSlab;
+  const uint32_t v_tiles = sm.v + (FP8 ? piece16 >> 2 : piece16 >> 3) * S::kSlab;
+  const int64_t block_bytes = (int64_t)a.Hkv * 16 * RB;
+  int kc = 0;
+  for (int64_t u = u0; u < u_end;) {
+    const Segment g = segment_at(a, pre, u, u_end, piece, *sm.abort_flag != 0);
+    u += g.units;
+    if (g.nt == 0) continue;
+    const int blocks = (g.len + 15) >> 4;
+    const int64_t first_row = (a.layer_blocks * a.Hkv + g.h) * 16;
+    const uint8_t* k_base = a.k + first_row * RB + piece16 * 16;
+    const int64_t v_minus_k = a.v - a.k;
+    // Blocks past the end read the last one (hidden, and zeroed where it would
+    // matter).
+    auto fetch_pages = [&](int kt) {
+      return __ldg(g.table + min((g.k0 + kt) * 8 + (lane & 7), blocks - 1));
+    };
+    auto load_row = [&](const uint8_t* base, int i, int pages) {
+      const int tok = token_of(i);
+      const int page = __shfl_sync(0xffffffffu, pages, tok >> 4);
+      return ldg_stream16(base + page * block_bytes + (tok & 15) * RB);
+    };
+    // Scales of tokens 4 lane .. 4 lane + 3 of a tile.
+    auto load_scales = [&](const float* from, int pages) {
+      const int64_t page = __shfl_sync(0xffffffffu, pages, lane >> 2);
+      return __ldg(reinterpret_cast<const float4*>(from + first_row + page * a.Hkv * 16) +
+                   (lane & 3));
+    };
+    uint4 kb[NI], vb[NI];
+    float4 ks = make_float4(0.f, 0.f, 0.f, 0.f), vs = ks;
+    // Page numbers run ahead of the rows they lead to.
+    int pages = fetch_pages(0), next_pages = fetch_pages(1);
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      kb[i] = load_row(k_base, i, pages);
+      vb[i] = load_row(k_base + v_minus_k, i, pages);
+    }
+    if constexpr (FP8) {
+      ks = load_scales(a.ks, pages);
+      vs = load_scales(a.vs, pages);
+    }
+    for (int kt = 0; kt < g.nt; ++kt, ++kc) {
+      const int st = kc & 1;
+      const uint32_t parity = ((kc >> 1) + 1) & 1;
+      const bool more = kt + 1 < g.nt;
+      const int later_pages = fetch_pages(kt + 2);
+      const int pos0 = (g.k0 + kt) * kTok;
+      const bool tail = pos0 + kTok > g.ctx;
+      if constexpr (FP8) {
+        float kx[4] = {ks.x, ks.y, ks.z, ks.w}, vx[4] = {vs.x, vs.y, vs.z, vs.w};
+        uint32_t top = 0u;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          // A row past the end gets the scale 0.  A key one of whose scales is not
+          // a number gets NaN scores and a value of zero, so that only the rows
+          // that see it get NaN.
+          const bool fine = isfinite(kx[e]) && isfinite(vx[e]);
+          if (!fine) kx[e] = __int_as_float(0x7fc00000);
+          if (!fine || (tail && pos0 + 4 * lane + e >= g.len)) vx[e] = 0.f;
+          top = max(top, __float_as_uint(vx[e]));
+        }
+        // Reference 2^(x - 126) > the tile's largest scale.  x is kept from 43 on
+        // (2^-83; 127 without any scale): sums of weights over the reference stay
+        // far from overflow then, even for heads whose values are all zero.
+        top = __reduce_max_sync(0xffffffffu, top);
+        const int x = top == 0u ? 127 : max(43, (int)(top >> 23));
+        const float factor = __int_as_float((253 - x) << 23) * 16384.f;  // 2^14 / reference
+        uint32_t pair[4];  // each token's scale over the reference as two fp16 numbers
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float y = vx[e] * factor;
+          pair[e] = pack_f16(y, y - __half2float(__float2half_rn(y)));
+        }
+        __syncwarp();
+        sts128(sm.pairs + lane * 16, pair[0], pair[1], pair[2], pair[3]);
+        __syncwarp();
+        if (group == 0 && cw == 0) {
+          const int slot = kc & (kTileBufs - 1);
+          reinterpret_cast<float4*>(sm.k_scale + slot * kTok)[lane] =
+              make_float4(kx[0], kx[1], kx[2], kx[3]);
+          if (lane == 0) sm.v_ref[slot] = (float)(x - 126 - 6);
+          mbar_arrive(sm.r_full + slot);
+        }
+        if (more) {
+          ks = load_scales(a.ks, next_pages);
+          vs = load_scales(a.vs, next_pages);
+        }
+      }
+      if (kc >= 2 && !warp_wait(sm.k_free + st, parity, a.status, sm.abort_flag)) break;
+      const uint32_t k_dst = k_tiles + st * S::kKTile;
+#pragma unroll
+      for (int part = 0; part < PARTS; ++part)
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+          const int tok = token_of(part * NI + i);
+          const uint4 w = kb[i];
+          if (part + 1 < PARTS) kb[i] = load_row(k_base, (part + 1) * NI + i, pages);
+          else if (more) kb[i] = load_row(k_base, i, next_pages);
+          sts128(k_dst + tok * 128 + ((k_chunk ^ (tok & 7)) << 4), w.x, w.y, w.z, w.w);
+        }
+      fence_proxy_async_smem();
+      mbar_arrive(sm.k_full + st);
+      if (kc >= 2 && !warp_wait(sm.v_free + st, parity, a.status, sm.abort_flag)) break;
+      const uint32_t v_dst = v_tiles + st * S::kVTile;
+#pragma unroll
+      for (int part = 0; part < PARTS; ++part)
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+          const int tok = token_of(part * NI + i);
+          uint32_t w[4] = {vb[i].x, vb[i].y, vb[i].z, vb[i].w};
+          if (part + 1 < PARTS) vb[i] = load_row(k_base + v_minus_k, (part + 1) * NI + i, pages);
+          else if (more) vb[i] = load_row(k_base + v_minus_k, i, next_pages);
+          const uint32_t c0 = v_dst + tok * 128 + ((v_chunk ^ (tok & 7)) << 4);
+          if constexpr (FP8) {
+            // Codes unpack times 2^-8, scales are at most 2^14: 448 x 2^6 at most.
+            const uint32_t pair = lds32(sm.pairs + tok * 4);
+            const uint32_t hi = __byte_perm(pair, 0u, 0x1010), lo = __byte_perm(pair, 0u, 0x3232);
+            uint32_t f[8];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) e4m3_to_f16(w[j], f[2 * j], f[2 * j + 1]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) f[j] = hfma2(f[j], hi, hmul2(f[j], lo));
+            sts128(c0, f[0], f[1], f[2], f[3]);
+            sts128(c0 ^ 16u, f[4], f[5], f[6], f[7]);
+          } else {
+            if (tail) {
+              // Value rows that a product must not meet: past the end anything may
+              // lie there, and a node may hold an infinity or a NaN that its
+              // siblings do not see (added to the rows that do see it at the end).
+              bool bad = false;
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                if (pos0 + tok >= g.len) w[j] = 0u;
+                if ((w[j] & 0x7f80u) == 0x7f80u) { w[j] &= 0xffff0000u; bad = true; }
+                if ((w[j] & 0x7f800000u) == 0x7f800000u) { w[j] &= 0xffffu; bad = true; }
+              }
+              if (bad) *sm.nonfinite = 1;
+            }
+            sts128(c0, w[0], w[1], w[2], w[3]);
+          }
+        }
+      fence_proxy_async_smem();
+      mbar_arrive(sm.v_full + st);
+      pages = next_pages;
+      next_pages = later_pages;
+    }
+  }
+}
+
 template <int D, bool FP8>
 __global__ void __launch_bounds__(kTileThreads, 1) attn_tiles_kernel(const Args a) {
-  using S = TileSmem<D>;
-  constexpr int RB = FP8 ? D : 2 * D;       // bytes of a cache row
-  constexpr int LPT = RB / 16;              // lanes that share a row, 16 bytes each
-  constexpr int NI = LPT;                   // 16-byte loads of a lane for one tile
-  constexpr int TPW = 32 / LPT;             // rows of one warp-wide load
-  constexpr uint32_t kSlab = 128 * 128;     // 64 values of 128 rows
-  constexpr float kUp = FP8 ? 7.f : 0.f;    // weights are held as 2^kUp w
+  using S = TileSmem<D, FP8>;
+  constexpr uint32_t kSlab = S::kSlab;
+  constexpr float kUp = FP8 ? 7.f : 0.f;  // weights are held as 2^kUp w
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
-  float* scales = reinterpret_cast<float*>(smem + S::kScales);
+  float* k_scale = reinterpret_cast<float*>(smem + S::kScale);
   float* sm_ml = reinterpret_cast<float*>(smem + S::kMl);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kBars);
   uint64_t* k_full = bars;        // [2]
   uint64_t* v_full = bars + 2;    // [2]
   uint64_t* k_free = bars + 4;    // [2]
   uint64_t* v_free = bars + 6;    // [2]
-  uint64_t* s_full = bars + 8;    // [2]
-  uint64_t* p_full = bars + 10;   // [2]
-  uint64_t* pv_done = bars + 12;  // [2]
-  uint64_t* sc_full = bars + 14;  // [kScaleBufs]
+  uint64_t* s_full = bars + 8;    // [group][2]
+  uint64_t* p_full = bars + 12;   // [group][2]
+  uint64_t* pv_done = bars + 16;  // [group][2]
+  uint64_t* r_full = bars + 20;   // [kTileBufs]: a tile's scale references
+  uint64_t* q_full = r_full + kTileBufs;
   int64_t* pre = reinterpret_cast<int64_t*>(smem + S::kPre);
   __shared__ int64_t s_sum[kTileThreads / 32];
+  __shared__ float s_vref[kTileBufs];
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort, s_last, s_nonfinite;
 
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = tid >> 5;
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(k_full + i, 128);
-      mbar_init(v_full + i, 128);
-      mbar_init(k_free + i, 1);
-      mbar_init(v_free + i, 1);
+      mbar_init(k_full + i, 256);
+      mbar_init(v_full + i, 256);
+      mbar_init(k_free + i, 2);
+      mbar_init(v_free + i, 2);
+    }
+    for (int i = 0; i < 4; ++i) {
       mbar_init(s_full + i, 1);
       mbar_init(p_full + i, 128);
       mbar_init(pv_done + i, 1);
     }
-    for (int i = 0; i < kScaleBufs; ++i) mbar_init(sc_full + i, 128);
+    for (int i = 0; i < kTileBufs; ++i) mbar_init(r_full + i, 32);
+    mbar_init(q_full, 256);
     fence_mbar_init();
     s_abort = 0;
+    s_nonfinite = 0;
   }
   // Tensor memory is taken only once the kernels before are done, and the next
   // one is let in only then: neither ever waits for columns the other holds.
   grid_dep_wait();
-  if (warp == 12) {
+  if (warp == 16) {
     tmem_alloc(&s_tmem, 512);
     tmem_relinquish();
   }
+  scan_work<kTok, kTileThreads>(a, kTileRows, pre, s_sum);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = s_tmem;
   grid_dep_launch();
 
-  scan_work<kTok, kTileThreads>(a, kTileRows, pre, s_sum);
   const int64_t total = pre[a.B];
   const int64_t piece = max((int64_t)1, (total + gridDim.x - 1) / gridDim.x);
-  int64_t u = (int64_t)blockIdx.x * piece;
-  const int64_t u_end = min(total, u + piece);
+  const int64_t u0 = (int64_t)blockIdx.x * piece;
+  const int64_t u_end = min(total, u0 + piece);
   volatile int* abort_flag = &s_abort;
 
-  int kc0 = 0;              // K / V tiles of earlier segments
-  int done[2] = {0, 0};     // products O += P V of each group so far
-
-  while (u < u_end) {
-    const int b = find_seq(pre, a.B, u);
-    const SeqShape s = seq_shape<kTok>(a, b, kTileRows);
-    const int64_t local = u - pre[b];
-    const int job = (int)(local / s.nb);
-    const int k0 = (int)(local - (int64_t)job * s.nb);
-    const int k1 = (int)min((int64_t)s.nb, k0 + (u_end - u));
-    const int h = job / s.tiles, tile = job - h * s.tiles;
-    const int ctx = s.len - s.n;
-    const int* table = a.table + (int64_t)b * a.table_stride;
-    const int q_row0 = a.row_start[b];
-    const int rows = min(kTileRows, s.n * a.G - tile * kTileRows);
-    const int mt = rows > 128 ? 2 : 1;
-    const int blocks = (s.len + 15) >> 4;
-    int nt = max(0, min(k1, (s.len + kTok - 1) / kTok) - k0);
-    if (*abort_flag) nt = 0;
-    const int ns = nt * mt;
-
-    // This softmax thread's row, and its query row in shared memory.
-    const int wg = warp >> 2;
-    const int row = mt == 2 ? tid : tid & 127;
-    const bool live_row = warp < 8 && row < rows;
-    const int rr = tile * kTileRows + (live_row ? row : 0);
-    const int node = rr / a.G;
-    const int64_t q_row = q_row0 + node;
-    const int head = h * a.G + rr % a.G;
-    float row_scale = a.scale_log2;
-    if (warp < 8) {
-      uint4 y[D / 8];
-      const __nv_bfloat16* qp = a.q + q_row * a.q_stride + (int64_t)head * D;
-      uint32_t top = 0;
+  if (warp >= 16) {
+    // -------------------------------------------------------------- products
+    // Warps 16, 17: scores of the two groups; 18, 19: their sums.  (One warp for all
+    // took longer to issue than the products to run.)  A warp walks through its
+    // steps together, on values that are the same in every lane: the product
+    // instructions take their operands from uniform registers (45 cycles each
+    // this way, 110 from one lane's own).  One lane issues.
+    fewer_registers<kRegsIssue>();
+    auto same = [](int v) { return __shfl_sync(0xffffffffu, v, 0); };
+    const int w = same(warp & 1), is_sum = same((warp >> 1) & 1);
+    const uint32_t tm = (uint32_t)same((int)tmem);
+    // (addresses stay below 2^18: offsets add to a descriptor's address field)
+    const uint64_t q_desc = umma_desc_sw128((uint32_t)same((int)smem_u32(smem + S::kQ)));
+    const uint64_t k_desc = umma_desc_sw128((uint32_t)same((int)smem_u32(smem + S::kK)));
+    const uint64_t v_desc = desc_v((uint32_t)same((int)smem_u32(smem + S::kV)), kSlab);
+    const bool issuer = elect_one();
+    uint64_t* const s_bar = s_full + 2 * w;
+    uint64_t* const p_bar = p_full + 2 * w;
+    uint64_t* const pv_bar = pv_done + 2 * w;
+    int kc0 = 0, seg = 0, n = 0;  // tiles, segments and this group's steps so far
+    for (int64_t u = u0; u < u_end;) {
+      const Segment g = segment_at(a, pre, u, u_end, piece, *abort_flag != 0);
+      u += g.units;
+      const int nt = same(g.nt), two = same(g.mt == 2 ? 1 : 0);
+      if (nt == 0) continue;
+      const int steps = same(kSpt * group_tiles(nt, two + 1, w));
+      if (!is_sum) {
+        if (!warp_wait(q_full, seg++ & 1, a.status, abort_flag)) continue;
+        const uint64_t qd = q_desc + (uint32_t)((w & two) * (S::kQTile >> 4));
+        for (int j = 0; j < steps; ++j, ++n) {
+          const int kc = kc0 + (two ? j / kSpt : w + j / kSpt * 2), sg = kc & 1;
+          const int buf = n % kSb, part = j % kSpt;
+          // The scores take the place of the weights of kSb steps before.
+          if (j >= kSb && !warp_wait(pv_bar + buf, (n / kSb + 1) & 1, a.status, abort_flag)) break;
+          if (part == 0 && !warp_wait(k_full + sg, (kc >> 1) & 1, a.status, abort_flag)) break;
+          tc_fence_after();
+          const uint64_t kd =
+              k_desc + (uint32_t)(sg * (S::kKTile >> 4) + part * (kStep * 128 >> 4));
+          const uint32_t d = tm + w * 128 + buf * kStep;
+          if (issuer) {
 #pragma unroll
-      for (int c = 0; c < D / 8; ++c) {
-        y[c] = live_row ? *reinterpret_cast<const uint4*>(qp + 8 * c) : make_uint4(0u, 0u, 0u, 0u);
-        if constexpr (FP8) {
-          const uint32_t w[4] = {y[c].x, y[c].y, y[c].z, y[c].w};
+            for (int ks = 0; ks < D / 16; ++ks) {
+              if constexpr (FP8) {  // first the high parts of q, then the low ones
+                const int half = ks / (D / 32), kk = ks % (D / 32);
+                mma_e4m3_ss(d, qd + ((half * kSlab + kk * 32) >> 4), kd + (kk * 32 >> 4),
+                            idesc(0, kStep, false), ks != 0);
+              } else {
+                const uint32_t off = ((ks >> 2) * kSlab + (ks & 3) * 32) >> 4;
+                mma_bf16_ss(d, qd + off, kd + off, idesc(1, kStep, false), ks != 0);
+              }
+            }
+            mma_commit(s_bar + buf);
+            if (part == kSpt - 1) {  // two arrivals free a tile: one of each reading group
+              mma_commit(k_free + sg);
+              if (!two) mma_commit(k_free + sg);
+            }
+          }
+          __syncwarp();
+        }
+      } else {
+        for (int j = 0; j < steps; ++j, ++n) {
+          const int kc = kc0 + (two ? j / kSpt : w + j / kSpt * 2), sg = kc & 1;
+          const int buf = n % kSb, part = j % kSpt;
+          if (part == 0 && !warp_wait(v_full + sg, (kc >> 1) & 1, a.status, abort_flag)) break;
+          if (!warp_wait(p_bar + buf, (n / kSb) & 1, a.status, abort_flag)) break;
+          tc_fence_after();
+          const uint64_t vd =
+              v_desc + (uint32_t)(sg * (S::kVTile >> 4) + part * (kStep * 128 >> 4));
+          const uint32_t d = tm + 256 + w * 128, p = tm + w * 128 + buf * kStep;
+          if (issuer) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            top = max(top, max(w[i] & 0x7fffu, (w[i] >> 16) & 0x7fffu));
+            for (int ks = 0; ks < kStep / 16; ++ks)
+              mma_bf16_ts(d, p + ks * 8, vd + ks * (2048 >> 4), idesc(FP8 ? 0 : 1, D, true),
+                          j > 0 || ks != 0);
+            mma_commit(pv_bar + buf);
+            if (part == kSpt - 1) {
+              mma_commit(v_free + sg);
+              if (!two) mma_commit(v_free + sg);
+            }
+          }
+          __syncwarp();
         }
       }
-      float up = 1.f;
-      if constexpr (FP8) {
-        const int e = (int)(top >> 7);
-        const int sh = e == 0 || e == 255 ? 0 : min(100, 127 + 14 - e);
-        up = __int_as_float((127 + sh) << 23);
-        row_scale *= __int_as_float((127 - sh) << 23);
-      }
-      if (mt == 2 || wg == 0) {
-        const uint32_t dst = smem_u32(smem + S::kQ) + (mt == 2 ? wg : 0) * S::kOperand;
-        const int r = tid & 127;
+      kc0 += nt;
+    }
+    __syncwarp();
+  } else if (warp >= 8) {
+    fewer_registers<kRegsLoad>();
+    LoadSmem sm;
+    sm.k = smem_u32(smem + S::kK);
+    sm.v = smem_u32(smem + S::kV);
+    sm.pairs = smem_u32(smem + S::kPairs) + (warp - 8) * kTok * 4;
+    sm.k_scale = k_scale;
+    sm.v_ref = s_vref;
+    sm.k_full = k_full;
+    sm.v_full = v_full;
+    sm.k_free = k_free;
+    sm.v_free = v_free;
+    sm.r_full = r_full;
+    sm.abort_flag = abort_flag;
+    sm.nonfinite = &s_nonfinite;
+    load_tiles<D, FP8>(a, pre, u0, u_end, piece, sm, (warp - 8) >> 2);
+  } else {
+    // -------------------------------------------------------------- softmax
+    more_registers<kRegsSoftmax>();
+    const int wg = warp >> 2;
+    const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t o_addr = lane_base + 256 + wg * 128;
+    int kc0 = 0, n = 0;  // tiles and this group's steps so far
+    for (int64_t u = u0; u < u_end;) {
+      const Segment g = segment_at(a, pre, u, u_end, piece, *abort_flag != 0);
+      u += g.units;
+      // This thread's row, its query into shared memory.
+      const int row = g.mt == 2 ? tid : tid & 127;
+      const bool live_row = row < g.rows;
+      const bool live_warp = (g.mt == 2 ? warp : warp & 3) * 32 < g.rows;
+      const int rr = g.row0 + (live_row ? row : 0);
+      const int node = rr / a.G;
+      const int64_t q_row = g.q_row0 + node;
+      const int head = g.h * a.G + rr % a.G;
+      float row_scale = a.scale_log2;
+      {
+        uint4 y[D / 8];
+        const __nv_bfloat16* qp = a.q + q_row * a.q_stride + (int64_t)head * D;
+        uint32_t top = 0;
 #pragma unroll
-        for (int c = 0; c < D / 8; ++c) {
-          uint32_t w[4] = {y[c].x, y[c].y, y[c].z, y[c].w};
-          if constexpr (FP8) {
+        for (int c = 0; c < D / 8; ++c)
+          y[c] = live_row ? *reinterpret_cast<const uint4*>(qp + 8 * c) : make_uint4(0u, 0u, 0u, 0u);
+        const bool writes = g.mt == 2 || wg == 0;
+        const uint32_t dst =
+            smem_u32(smem + S::kQ) + (g.mt == 2 ? wg : 0) * S::kQTile + (tid & 127) * 128;
+        const int r = tid & 7;
+        if constexpr (FP8) {
+          // A power of two that puts the row's largest value into [2^7, 2^8).
+#pragma unroll
+          for (int c = 0; c < D / 8; ++c) {
+            const uint32_t w[4] = {y[c].x, y[c].y, y[c].z, y[c].w};
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              w[i] = pack_f16(__uint_as_float(w[i] << 16) * up,
-                              __uint_as_float(w[i] & 0xffff0000u) * up);
+              top = max(top, max(w[i] & 0x7fffu, (w[i] >> 16) & 0x7fffu));
           }
-          sts128(dst + (c >> 3) * kSlab + r * 128 + (((c & 7) ^ (r & 7)) << 4), w[0], w[1], w[2],
-                 w[3]);
+          const int e = (int)(top >> 7);
+          const int sh = e == 0 || e == 255 ? 0 : min(100, 127 + 7 - e);
+          const float up = __int_as_float((127 + sh) << 23);
+          row_scale *= __int_as_float((127 - sh) << 23);
+          if (e == 255) row_scale = __int_as_float(0x7fc00000);  // an infinity or a NaN in the row
+#pragma unroll
+          for (int c = 0; c < D / 8; c += 2) {
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {  // 4 dims a word
+              const uint4& z = y[c + (i >> 1)];
+              const uint32_t a0 = i & 1 ? z.z : z.x, a1 = i & 1 ? z.w : z.y;
+              const float x[4] = {__uint_as_float(a0 << 16) * up,
+                                  __uint_as_float(a0 & 0xffff0000u) * up,
+                                  __uint_as_float(a1 << 16) * up,
+                                  __uint_as_float(a1 & 0xffff0000u) * up};
+              hi[i] = lo[i] = 0u;
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                const uint32_t h8 = __nv_cvt_float2_to_fp8x2(make_float2(x[2 * k], x[2 * k + 1]),
+                                                             __NV_SATFINITE, __NV_E4M3);
+                const float2 back = __half22float2(
+                    __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)h8, __NV_E4M3));
+                const uint32_t l8 = __nv_cvt_float2_to_fp8x2(
+                    make_float2(x[2 * k] - back.x, x[2 * k + 1] - back.y), __NV_SATFINITE,
+                    __NV_E4M3);
+                hi[i] |= h8 << (16 * k);
+                lo[i] |= l8 << (16 * k);
+              }
+            }
+            if (writes) {
+              const uint32_t at = dst + (((c >> 1) ^ r) << 4);
+              sts128(at, hi[0], hi[1], hi[2], hi[3]);
+              sts128(at + kSlab, lo[0], lo[1], lo[2], lo[3]);
+            }
+          }
+        } else if (writes) {
+#pragma unroll
+          for (int c = 0; c < D / 8; ++c)
+            sts128(dst + (c >> 3) * kSlab + (((c & 7) ^ r) << 4), y[c].x, y[c].y, y[c].z, y[c].w);
         }
+        fence_proxy_async_smem();
+        tc_fence_before();
+        if (g.nt > 0) mbar_arrive(q_full);
       }
-      fence_proxy_async_smem();
-    }
-    if (tid == 0) s_nonfinite = 0;
-    __syncthreads();
-
-    float m = kNegBig, l = 0.f;
-    if (warp < 8) {
-      // ------------------------------------------------------------ softmax
-      const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-      const uint32_t s_addr = lane_base + wg * 128;
-      const uint32_t o_addr = lane_base + 256 + wg * 128;
-      const bool live_warp = (mt == 2 ? warp : warp & 3) * 32 < rows;
       RowSight sight;
-      sight.len = s.len;
-      sight.ctx = ctx;
+      sight.len = g.len;
+      sight.ctx = g.ctx;
       sight.node = node;
       sight.masked = a.masks != nullptr;
       sight.mask = sight.masked && live_row ? (uint64_t)a.masks[q_row] : 0;
-      int n = done[wg];
-      for (int st = wg; st < ns; st += 2) {
-        const int kt = mt == 2 ? st >> 1 : st;
+
+      float m = kNegBig, l = 0.f;
+      const int tiles = group_tiles(g.nt, g.mt, wg);
+      bool ok = true;
+      for (int j = 0; j < kSpt * tiles; ++j, ++n) {
+        const int kt = g.mt == 2 ? j / kSpt : wg + j / kSpt * 2;
+        const int buf = n % kSb;
         const int kc = kc0 + kt;
-        const int pos0 = (k0 + kt) * kTok;
-        if (!warp_wait(s_full + wg, n & 1, a.status, abort_flag)) break;
-        if (!warp_wait(sc_full + (kc & (kScaleBufs - 1)), (kc / kScaleBufs) & 1, a.status,
-                       abort_flag))
-          break;
+        const int pos0 = (g.k0 + kt) * kTok + j % kSpt * kStep;
+        const uint32_t s_addr = lane_base + wg * 128 + buf * kStep;
+        ok = warp_wait(s_full + 2 * wg + buf, (n / kSb) & 1, a.status, abort_flag) &&
+             (!FP8 || j % kSpt != 0 || warp_wait(r_full + (kc & (kTileBufs - 1)), (kc / kTileBufs) & 1, a.status,
+                                   abort_flag));
+        if (!ok) break;
         tc_fence_after();
-        bool ok = true;
         if (live_warp) {
-          const float* sc = scales + (kc & (kScaleBufs - 1)) * 3 * kTok;
-          const bool tail = pos0 + kTok > ctx;
-          // Scores of columns c .. c + 3 in base 2, with log2 of the values'
-          // scales added.
-          auto score4 = [&](float* v, int c) {
-            if constexpr (FP8) {
-              const float4 k4 = *reinterpret_cast<const float4*>(sc + c);
-              const float4 l4 = *reinterpret_cast<const float4*>(sc + kTok + c);
-              v[0] = fmaf(v[0] * k4.x, row_scale, l4.x);
-              v[1] = fmaf(v[1] * k4.y, row_scale, l4.y);
-              v[2] = fmaf(v[2] * k4.z, row_scale, l4.z);
-              v[3] = fmaf(v[3] * k4.w, row_scale, l4.w);
-            } else {
+          // Score in base 2, with log2 of the values' reference, less `shift`.
+          const float mul = row_scale;
+          const float lv = FP8 ? s_vref[kc & (kTileBufs - 1)] : 0.f;
+          const float* sc = k_scale + (kc & (kTileBufs - 1)) * kTok + j % kSpt * kStep;
+          const bool tail = pos0 + kStep > g.ctx;
+          bool again = __any_sync(0xffffffffu, tail || m == kNegBig);
+          float sum = 0.f;
+          if (!again) {
+            const F2 mul2v = f2(mul, mul);
+            const float shift = lv + kUp - m;
+            const F2 shift2 = f2(shift, shift);
+            F2 sum2 = f2(0.f, 0.f);
+            float mx = -INFINITY;
+            uint32_t p[kStep / 2];
+            uint32_t v[2][32];
+            tmem_ld32_start(s_addr, v[0]);
 #pragma unroll
-              for (int i = 0; i < 4; ++i) v[i] *= row_scale;
-            }
-          };
-          float mx = -INFINITY;
+            for (int c = 0; c < kStep / 32; ++c) {
+              tmem_ld32_wait(v[c & 1]);
+              if (c + 1 < kStep / 32) tmem_ld32_start(s_addr + 32 * (c + 1), v[(c + 1) & 1]);
 #pragma unroll
-          for (int c0 = 0; c0 < kTok; c0 += 32) {
-            float v[32];
-            __syncwarp();
-            tmem_ld32(s_addr + c0, v);
-            const uint32_t seen = tail ? sight.at(pos0 + c0) : 0xffffffffu;
+              for (int i = 0; i < 32; i += 4) {
+                const uint32_t* y = v[c & 1] + i;
+                F2 x0 = f2(__uint_as_float(y[0]), __uint_as_float(y[1]));
+                F2 x1 = f2(__uint_as_float(y[2]), __uint_as_float(y[3]));
+                if constexpr (FP8) {
+                  const float4 k4 = *reinterpret_cast<const float4*>(sc + 32 * c + i);
+                  x0 = mul2(x0, f2(k4.x, k4.y));
+                  x1 = mul2(x1, f2(k4.z, k4.w));
+                }
+                x0 = fma2(x0, mul2v, shift2);
+                x1 = fma2(x1, mul2v, shift2);
+                float t[4];
+                split(x0, t[0], t[1]);
+                split(x1, t[2], t[3]);
+                mx = fmaxf(fmaxf(mx, fmaxf(t[0], t[1])), fmaxf(t[2], t[3]));
 #pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-              score4(v + i, c0 + i);
-              if (tail) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[i + e] = seen >> (i + e) & 1 ? v[i + e] : -INFINITY;
+                for (int e = 0; e < 4; ++e) t[e] = ex2(t[e]);
+                sum2 = add2(sum2, add2(f2(t[0], t[1]), f2(t[2], t[3])));
+                p[16 * c + i / 2] = FP8 ? pack_f16(t[0], t[1]) : pack_bf16(t[0], t[1]);
+                p[16 * c + i / 2 + 1] = FP8 ? pack_f16(t[2], t[3]) : pack_bf16(t[2], t[3]);
               }
-              mx = fmaxf(mx, fmaxf(fmaxf(v[i], v[i + 1]), fmaxf(v[i + 2], v[i + 3])));
+            }
+            again = __any_sync(0xffffffffu, mx > 8.f + kUp);
+            if (!again) {
+#pragma unroll
+              for (int c = 0; c < kStep / 2; c += 16) {
+                uint32_t w[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) w[i] = p[c + i];
+                tmem_st16(s_addr + c, w);
+              }
+              float s0, s1;
+              split(sum2, s0, s1);
+              sum = s0 + s1;
             }
           }
-          float alpha = 1.f;
-          if (mx > m + 8.f) {
-            alpha = ex2(m - mx);
-            m = mx;
-            l *= alpha;
-          }
-          if (__any_sync(0xffffffffu, alpha != 1.f) && st >= 2) {
-            ok = warp_wait(pv_done + wg, (n - 1) & 1, a.status, abort_flag);
-            if (ok) {
-              tc_fence_after();
+          if (again) {
+            // Two passes: the step's maximum first.
+            auto scaled = [&](uint32_t acc, int c) {
+              return FP8 ? __uint_as_float(acc) * sc[c] : __uint_as_float(acc);
+            };
+            float mx = -INFINITY;
+#pragma unroll 1
+            for (int c0 = 0; c0 < kStep; c0 += 32) {
+              uint32_t v[32];
+              __syncwarp();
+              tmem_ld32_start(s_addr + c0, v);
+              tmem_ld32_wait(v);
+              const uint32_t seen = tail ? sight.at(pos0 + c0) : 0xffffffffu;
 #pragma unroll
-              for (int c0 = 0; c0 < D; c0 += 32) {
-                float v[32];
-                tmem_ld32(o_addr + c0, v);
+              for (int i = 0; i < 32; ++i)
+                mx = fmaxf(mx, seen >> i & 1 ? fmaf(scaled(v[i], c0 + i), mul, lv) : -INFINITY);
+            }
+            float alpha = 1.f;
+            if (mx > m) {
+              alpha = ex2(m - mx);
+              m = mx;
+              l *= alpha;
+            }
+            if (__any_sync(0xffffffffu, alpha != 1.f) && j > 0) {
+              ok = warp_wait(pv_done + 2 * wg + (n - 1) % kSb, ((n - 1) / kSb) & 1, a.status,
+                             abort_flag);
+              tc_fence_after();
+#pragma unroll 1
+              for (int c0 = 0; c0 < D; c0 += 16) {
+                float v[16];
+                __syncwarp();
+                tmem_ld16(o_addr + c0, v);
                 uint32_t w[16];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(v[i] * alpha);
                 tmem_st16(o_addr + c0, w);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(v[16 + i] * alpha);
-                tmem_st16(o_addr + c0 + 16, w);
               }
-              tmem_st_wait();
+            }
+            const float shift = lv + kUp - m;
+            sum = 0.f;
+#pragma unroll 1
+            for (int c0 = 0; c0 < kStep; c0 += 32) {
+              uint32_t v[32];
+              __syncwarp();
+              tmem_ld32_start(s_addr + c0, v);
+              tmem_ld32_wait(v);
+              const uint32_t seen = tail ? sight.at(pos0 + c0) : 0xffffffffu;
+              uint32_t w[16];
+#pragma unroll
+              for (int i = 0; i < 32; i += 2) {
+                float t[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  t[e] = ex2(fmaf(scaled(v[i + e], c0 + i + e), mul, shift));
+                  if (!(seen >> (i + e) & 1)) t[e] = 0.f;
+                  sum += t[e];
+                }
+                w[i / 2] = FP8 ? pack_f16(t[0], t[1]) : pack_bf16(t[0], t[1]);
+              }
+              tmem_st16(s_addr + c0 / 2, w);
             }
           }
-          const float base = m - kUp;
-          float sum = 0.f;
-#pragma unroll
-          for (int c0 = 0; c0 < kTok; c0 += 32) {
-            float v[32];
-            __syncwarp();
-            tmem_ld32(s_addr + c0, v);
-            const uint32_t seen = tail ? sight.at(pos0 + c0) : 0xffffffffu;
-#pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-              score4(v + i, c0 + i);
-              alignas(16) float inv[4] = {1.f, 1.f, 1.f, 1.f};
-              if constexpr (FP8)
-                *reinterpret_cast<float4*>(inv) =
-                    *reinterpret_cast<const float4*>(sc + 2 * kTok + c0 + i);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                float w = ex2(v[i + e] - base);
-                float part = FP8 ? w * inv[e] : w;
-                // (a hidden key's scale may be a NaN)
-                if (tail && !(seen >> (i + e) & 1)) w = part = 0.f;
-                sum += part;
-                v[i + e] = w;
-              }
-            }
-            uint32_t p[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              if constexpr (FP8) {
-                p[i] = pack_f16(v[2 * i], v[2 * i + 1]);
-              } else {
-                const __nv_bfloat162 y = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-                p[i] = *reinterpret_cast<const uint32_t*>(&y);
-              }
-            }
-            tmem_st16(s_addr + c0 / 2, p);
-          }
-          l += sum;
+          // (the weights count the values' reference: 2^lv of it out again)
+          l += FP8 ? sum * ex2(-lv) : sum;
           tmem_st_wait();
         }
         if (!ok) break;
         tc_fence_before();
-        mbar_arrive(p_full + wg);
-        ++n;
+        mbar_arrive(p_full + 2 * wg + buf);
       }
-      if (n > done[wg]) warp_wait(pv_done + wg, (n - 1) & 1, a.status, abort_flag);
+      if (tiles > 0 && ok)
+        ok = warp_wait(pv_done + 2 * wg + (n - 1) % kSb, ((n - 1) / kSb) & 1, a.status, abort_flag);
       tc_fence_after();
-      // The groups' statistics, for joining.
-      sm_ml[(wg * 128 + (tid & 127)) * 2] = ns > wg ? m : kNegBig;
-      sm_ml[(wg * 128 + (tid & 127)) * 2 + 1] = ns > wg ? l : 0.f;
-    } else if (warp < 12) {
-      // ------------------------------------------------------------ K and V
-      const int ct = tid - 256, cw = ct >> 5;
-      const int piece16 = lane % LPT;
-      auto token_of = [&](int i) { return i * 4 * TPW + cw * TPW + lane / LPT; };
-      uint4 kb[NI];
-      uint4 vb[NI];  // (bf16 rows are twice as long: kb alone serves both)
-      float ks_r = 0.f, vs_r = 1.f;
-      int pages = 0;
-      auto fetch_pages = [&](int kt) {
-        const int blk = (k0 + kt) * 8 + lane;
-        return lane < 8 && blk < blocks ? __ldg(table + blk) : -1;
-      };
-      auto load = [&](uint4(&buf)[NI], const uint8_t* base, int kt) {
+      // Join the groups (one row tile) and the CTAs that share the job.
+      sm_ml[(wg * 128 + (tid & 127)) * 2] = m;
+      sm_ml[(wg * 128 + (tid & 127)) * 2 + 1] = l;
+      tc_fence_before();
+      named_bar_sync(2, 256);
+      tc_fence_after();
+      ok = ok && !*abort_flag;
+      const bool whole = g.c0 == g.c1;
+      const int64_t c0 = g.c0, c1 = g.c1;
+      // With one row tile each group joins and stores half of the dims.
+      const int d_lo = g.mt == 2 ? 0 : wg * (D / 2), d_hi = g.mt == 2 ? D : d_lo + D / 2;
+      float* slot = a.part + ((int64_t)blockIdx.x * 2 + (blockIdx.x == c0 ? 1 : 0)) * kTileRows *
+                                 (D + 2);
+      auto put = [&](int d, float (&y)[16], float inv, bool none) {
+        uint32_t w[8];
 #pragma unroll
-        for (int i = 0; i < NI; ++i) {
-          const int tok = token_of(i);
-          const int page = __shfl_sync(0xffffffffu, pages, tok >> 4);
-          buf[i] = page >= 0 ? ldg_stream16(base + (((a.layer_blocks + page) * a.Hkv + h) * 16 +
-                                                    (tok & 15)) * RB + piece16 * 16)
-                             : make_uint4(0u, 0u, 0u, 0u);
+        for (int i = 0; i < 16; ++i) y[i] = none ? 0.f : y[i] * inv;
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+          // (8-bit values come with dims 0, 2, 1, 3 of every four)
+          w[i / 2] = FP8 ? pack_bf16(y[i], y[i + 2]) : pack_bf16(y[i], y[i + 1]);
+          w[i / 2 + 1] = FP8 ? pack_bf16(y[i + 1], y[i + 3]) : pack_bf16(y[i + 2], y[i + 3]);
         }
-      };
-      auto load_scales = [&](int kt) {
-        if constexpr (FP8) {
-          const int page = __shfl_sync(0xffffffffu, pages, ct >> 4);
-          const bool there = page >= 0 && (k0 + kt) * kTok + ct < s.len;
-          const int64_t r = ((a.layer_blocks + page) * a.Hkv + h) * 16 + (ct & 15);
-          ks_r = there ? __ldg(a.ks + r) : 0.f;
-          vs_r = there ? __ldg(a.vs + r) : 1.f;
-        }
-      };
-      auto store = [&](const uint4(&buf)[NI], uint32_t dst) {
-#pragma unroll
-        for (int i = 0; i < NI; ++i) {
-          const int tok = token_of(i);
-          const uint32_t w[4] = {buf[i].x, buf[i].y, buf[i].z, buf[i].w};
-          if constexpr (FP8) {
-            uint32_t f[8];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              f[2 * j] = e4m3x2_to_f16x2(w[j] & 0xffffu);
-              f[2 * j + 1] = e4m3x2_to_f16x2(w[j] >> 16);
-            }
-            // Two chunks of 8 values; the lanes of the second slab start with
-            // the other one, which keeps the eight lanes of a phase on
-            // different banks.
-            const int c = 2 * piece16;
-            const uint32_t at = dst + (c >> 3) * kSlab + tok * 128;
-            const uint32_t c0 = at + (((c & 7) ^ (tok & 7)) << 4);
-            const uint32_t c1 = at + ((((c & 7) + 1) ^ (tok & 7)) << 4);
-            if (c >> 3) {
-              sts128(c1, f[4], f[5], f[6], f[7]);
-              sts128(c0, f[0], f[1], f[2], f[3]);
-            } else {
-              sts128(c0, f[0], f[1], f[2], f[3]);
-              sts128(c1, f[4], f[5], f[6], f[7]);
-            }
-          } else {
-            sts128(dst + (piece16 >> 3) * kSlab + tok * 128 +
-                       (((piece16 & 7) ^ (tok & 7)) << 4),
-                   w[0], w[1], w[2], w[3]);
-          }
-        }
-      };
-      // Value rows that a product must not meet: past the end anything may
-      // lie there, and a bf16 node may hold an infinity or a NaN that its
-      // siblings do not see (added to the rows that do see it at the end).
-      auto clean = [&](uint4(&buf)[NI], int kt) {
-        const int pos0 = (k0 + kt) * kTok;
-        if (pos0 + kTok <= ctx) return;
-#pragma unroll
-        for (int i = 0; i < NI; ++i) {
-          if (pos0 + token_of(i) >= s.len) buf[i] = make_uint4(0u, 0u, 0u, 0u);
-          if constexpr (!FP8) {
-            uint32_t w[4] = {buf[i].x, buf[i].y, buf[i].z, buf[i].w};
-            bool bad = false;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              if ((w[j] & 0x7f80u) == 0x7f80u) { w[j] &= 0xffff0000u; bad = true; }
-              if ((w[j] & 0x7f800000u) == 0x7f800000u) { w[j] &= 0xffffu; bad = true; }
-            }
-            if (bad) s_nonfinite = 1;
-            buf[i] = make_uint4(w[0], w[1], w[2], w[3]);
-          }
-        }
-      };
-      if (nt > 0) {
-        pages = fetch_pages(0);
-        load(kb, a.k, 0);
-        load_scales(0);
-        if constexpr (FP8) load(vb, a.v, 0);
-      }
-      for (int kt = 0; kt < nt; ++kt) {
-        const int kc = kc0 + kt, st = kc & 1;
-        const uint32_t parity = ((kc >> 1) + 1) & 1;
-        if (kc >= 2 && !warp_wait(k_free + st, parity, a.status, abort_flag)) break;
-        store(kb, smem_u32(smem + S::kK) + st * S::kOperand);
-        float* sc = scales + (kc & (kScaleBufs - 1)) * 3 * kTok;
-        if constexpr (FP8) {
-          const float lv = __log2f(vs_r);
-          sc[ct] = ks_r;
-          sc[kTok + ct] = lv;
-          sc[2 * kTok + ct] = ex2(-lv);
-        }
-        mbar_arrive(sc_full + (kc & (kScaleBufs - 1)));
-        fence_proxy_async_smem();
-        mbar_arrive(k_full + st);
-        if constexpr (FP8) {
-          if (kt + 1 < nt) {
-            pages = fetch_pages(kt + 1);
-            load(kb, a.k, kt + 1);
-            load_scales(kt + 1);
-          }
-        } else {
-          load(kb, a.v, kt);
-        }
-        if (kc >= 2 && !warp_wait(v_free + st, parity, a.status, abort_flag)) break;
-        if constexpr (FP8) {
-          clean(vb, kt);
-          store(vb, smem_u32(smem + S::kV) + st * S::kOperand);
-        } else {
-          clean(kb, kt);
-          store(kb, smem_u32(smem + S::kV) + st * S::kOperand);
-        }
-        fence_proxy_async_smem();
-        mbar_arrive(v_full + st);
-        if (kt + 1 < nt) {
-          if constexpr (FP8) {
-            load(vb, a.v, kt + 1);
-          } else {
-            pages = fetch_pages(kt + 1);
-            load(kb, a.k, kt + 1);
-          }
-        }
-      }
-    } else if (lane == 0) {
-      // ------------------------------------------------------------ products
-      int n[2] = {done[0], done[1]};
-      auto scores = [&](int st) {
-        const int g = st & 1, kt = mt == 2 ? st >> 1 : st, kc = kc0 + kt, sg = kc & 1;
-        if (!mbar_wait(k_full + sg, (kc >> 1) & 1, a.status, kStatusAttnTimeout, abort_flag))
-          return false;
-        tc_fence_after();
-        const uint32_t qa = smem_u32(smem + S::kQ) + (mt == 2 ? g : 0) * S::kOperand;
-        const uint32_t ka = smem_u32(smem + S::kK) + sg * S::kOperand;
-#pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) {
-          const uint32_t off = (ks >> 2) * kSlab + (ks & 3) * 32;
-          mma_bf16_ss(tmem + g * 128, umma_desc_sw128(qa + off), umma_desc_sw128(ka + off),
-                      idesc<FP8>(kTok, false), ks != 0);
-        }
-        mma_commit(s_full + g);
-        if (mt == 1 || g == 1) mma_commit(k_free + sg);
-        return true;
-      };
-      bool ok = true;
-      for (int st = 0; st < min(2, ns) && ok; ++st) ok = scores(st);
-      for (int st = 0; st < ns && ok; ++st) {
-        const int g = st & 1, kt = mt == 2 ? st >> 1 : st, kc = kc0 + kt, sg = kc & 1;
-        ok = mbar_wait(v_full + sg, (kc >> 1) & 1, a.status, kStatusAttnTimeout, abort_flag) &&
-             mbar_wait(p_full + g, n[g] & 1, a.status, kStatusAttnTimeout, abort_flag);
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t va = smem_u32(smem + S::kV) + sg * S::kOperand;
-#pragma unroll
-        for (int ks = 0; ks < kTok / 16; ++ks)
-          mma_bf16_ts(tmem + 256 + g * 128, tmem + g * 128 + ks * 8,
-                      desc_v(va + ks * 2048, kSlab), idesc<FP8>(D, true), st >= 2 || ks != 0);
-        mma_commit(pv_done + g);
-        if (mt == 1 || g == 1) mma_commit(v_free + sg);
-        if (st + 2 < ns) {
-          // The next scores overwrite the weights this product reads.
-          ok = mbar_wait(pv_done + g, n[g] & 1, a.status, kStatusAttnTimeout, abort_flag) &&
-               scores(st + 2);
-        }
-        ++n[g];
-      }
-    }
-    __syncwarp();
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-
-    // Join the groups (one row tile) and the CTAs that share the job.
-    const int64_t js = pre[b] + (int64_t)job * s.nb;
-    const int64_t c0 = js / piece, c1 = (js + s.nb - 1) / piece;
-    const bool whole = c0 == c1;
-    const bool ok = !*abort_flag;
-    // With one row tile each group joins and stores half of the dims.
-    const int d_lo = mt == 2 ? 0 : wg * (D / 2), d_hi = mt == 2 ? D : d_lo + D / 2;
-    float* slot = a.part + ((int64_t)blockIdx.x * 2 + (blockIdx.x == c0 ? 1 : 0)) * kTileRows *
-                               (D + 2);
-    const bool live_warp = warp < 8 && (mt == 2 ? warp : warp & 3) * 32 < rows;
-    auto put = [&](int d, const float (&y)[16]) {
-      __nv_bfloat16* dst = a.out + q_row * a.out_stride + (int64_t)head * D + d;
-      uint32_t w[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const __nv_bfloat162 p = __floats2bfloat162_rn(y[2 * i], y[2 * i + 1]);
-        w[i] = *reinterpret_cast<const uint32_t*>(&p);
-      }
-      if (a.out_vec) {
-        reinterpret_cast<uint4*>(dst)[0] = make_uint4(w[0], w[1], w[2], w[3]);
-        reinterpret_cast<uint4*>(dst)[1] = make_uint4(w[4], w[5], w[6], w[7]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          reinterpret_cast<uint16_t*>(dst)[2 * i] = (uint16_t)w[i];
-          reinterpret_cast<uint16_t*>(dst)[2 * i + 1] = (uint16_t)(w[i] >> 16);
-        }
-      }
-    };
-    if (live_warp && ok) {
-      const int r = tid & 127;
-      float f[2], M = m, L = l;
-      f[0] = f[1] = 0.f;
-      if (mt == 2) {
-        f[wg] = 1.f;
-        if (ns == 0) L = 0.f;
-      } else {
-        const float m0 = sm_ml[r * 2], m1 = sm_ml[(128 + r) * 2];
-        M = fmaxf(m0, m1);
-        f[0] = ex2(m0 - M);
-        f[1] = ex2(m1 - M);
-        L = sm_ml[r * 2 + 1] * f[0] + sm_ml[(128 + r) * 2 + 1] * f[1];
-      }
-      if (!whole && live_row && (mt == 2 || wg == 0)) {
-        slot[row] = M;
-        slot[kTileRows + row] = L;
-      }
-      const bool more = !FP8 && s_nonfinite;
-#pragma unroll 1
-      for (int d = d_lo; d < d_hi; d += 16) {
-        float y[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) y[i] = 0.f;
-#pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          if ((mt == 2 && g != wg) || ns <= g) continue;
-          float v[16];
-          __syncwarp();
-          tmem_ld16(tmem + ((uint32_t)((warp & 3) * 32) << 16) + 256 + g * 128 + d, v);
-#pragma unroll
-          for (int i = 0; i < 16; ++i) y[i] = fmaf(v[i], f[g], y[i]);
-        }
-        if (more && live_row) {
-          // The infinities and NaNs that were kept out of the products.
-          const bool masked = a.masks != nullptr;
-          const uint64_t mask = masked ? (uint64_t)a.masks[q_row] : 0;
-          for (int pos = max(k0, ctx / kTok) * kTok; pos < min(k1 * kTok, s.len); ++pos) {
-            const int j = pos - ctx;
-            if (j >= 0 && !(masked ? j < 64 && (mask >> (j & 63) & 1) : j <= node)) continue;
-            const int64_t vr = ((a.layer_blocks + table[pos >> 4]) * a.Hkv + h) * 16 + (pos & 15);
-            const __nv_bfloat16* vp = reinterpret_cast<const __nv_bfloat16*>(a.v) + vr * D + d;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float val = __bfloat162float(vp[i]);
-              if (!(fabsf(val) <= 3.4e38f)) y[i] += val;
-            }
-          }
-        }
-        if (!live_row) continue;
-        if (whole) {
-          const float inv = L == 0.f ? 0.f : 1.f / L;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) y[i] = L == 0.f ? 0.f : y[i] * inv;
-          put(d, y);
+        __nv_bfloat16* dst = a.out + q_row * a.out_stride + (int64_t)head * D + d;
+        if (a.out_vec) {
+          reinterpret_cast<uint4*>(dst)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+          reinterpret_cast<uint4*>(dst)[1] = make_uint4(w[4], w[5], w[6], w[7]);
         } else {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) slot[(2 + d + i) * kTileRows + row] = y[i];
+          for (int i = 0; i < 8; ++i) {
+            reinterpret_cast<uint16_t*>(dst)[2 * i] = (uint16_t)w[i];
+            reinterpret_cast<uint16_t*>(dst)[2 * i + 1] = (uint16_t)(w[i] >> 16);
+          }
         }
-      }
-    }
-    if (!whole) {
-      __threadfence();
-      __syncthreads();
-      if (tid == 0) {
-        s_last = atomicAdd(a.counters + c0, 1) == (int)(c1 - c0);
-        if (s_last) a.counters[c0] = 0;
-      }
-      __syncthreads();
-      if (s_last && live_row && ok) {
-        __threadfence();
-        auto part_of = [&](int64_t c) {
-          return a.part + (c * 2 + (c == c0 ? 1 : 0)) * kTileRows * (D + 2) + row;
-        };
-        float M = kNegBig, L = 0.f;
-        for (int64_t c = c0; c <= c1; ++c) M = fmaxf(M, __ldcg(part_of(c)));
-        for (int64_t c = c0; c <= c1; ++c)
-          L += __ldcg(part_of(c) + kTileRows) * ex2(__ldcg(part_of(c)) - M);
-        const float inv = L == 0.f ? 0.f : 1.f / L;
+      };
+      if (live_warp && ok) {
+        const int r = tid & 127;
+        float f[2] = {0.f, 0.f}, M = m, L = l;
+        if (g.mt == 2) {
+          f[wg] = 1.f;
+        } else {
+          const float m0 = sm_ml[r * 2], m1 = sm_ml[(128 + r) * 2];
+          M = fmaxf(m0, m1);
+          f[0] = ex2(m0 - M);
+          f[1] = ex2(m1 - M);
+          L = sm_ml[r * 2 + 1] * f[0] + sm_ml[(128 + r) * 2 + 1] * f[1];
+        }
+        if (!whole && live_row && (g.mt == 2 || wg == 0)) {
+          slot[row] = M;
+          slot[kTileRows + row] = L;
+        }
+        const bool more = !FP8 && *(volatile int*)&s_nonfinite;
 #pragma unroll 1
         for (int d = d_lo; d < d_hi; d += 16) {
           float y[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) y[i] = 0.f;
-          for (int64_t c = c0; c <= c1; ++c) {
-            const float* p = part_of(c);
-            const float f = ex2(__ldcg(p) - M);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) y[i] = fmaf(__ldcg(p + (2 + d + i) * kTileRows), f, y[i]);
+          for (int w = 0; w < 2; ++w) {
+            if ((g.mt == 2 && w != wg) || group_tiles(g.nt, g.mt, w) == 0) continue;
+            float v[16];
+            __syncwarp();
+            tmem_ld16(lane_base + 256 + w * 128 + d, v);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) y[i] = fmaf(v[i], f[w], y[i]);
           }
+          if (more && live_row) {
+            // The infinities and NaNs that were kept out of the products.
+            const int last = min((g.k0 + g.nt) * kTok, g.len);
+            for (int pos = max(g.k0, g.ctx / kTok) * kTok; pos < last; ++pos) {
+              if (!(sight.at(pos) & 1)) continue;
+              const int64_t vr =
+                  ((a.layer_blocks + g.table[pos >> 4]) * a.Hkv + g.h) * 16 + (pos & 15);
+              const __nv_bfloat16* vp = reinterpret_cast<const __nv_bfloat16*>(a.v) + vr * D + d;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) y[i] = L == 0.f ? 0.f : y[i] * inv;
-          put(d, y);
+              for (int i = 0; i < 16; ++i) {
+                const float val = __bfloat162float(vp[i]);
+                if (!(fabsf(val) <= 3.4e38f)) y[i] += val;
+              }
+            }
+          }
+          if (!live_row) continue;
+          if (whole) {
+            put(d, y, 1.f / L, L == 0.f);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) slot[(2 + d + i) * kTileRows + row] = y[i];
+          }
         }
       }
+      if (!whole) {
+        __threadfence();
+        named_bar_sync(2, 256);
+        if (tid == 0) {
+          s_last = atomicAdd(a.counters + c0, 1) == (int)(c1 - c0);
+          if (s_last) a.counters[c0] = 0;
+        }
+        named_bar_sync(2, 256);
+        if (s_last && live_row && ok) {
+          __threadfence();
+          constexpr int P = 4;  // parts whose loads are in flight together
+          auto part_of = [&](int64_t c) {
+            return a.part + (c * 2 + (c == c0 ? 1 : 0)) * kTileRows * (D + 2) + row;
+          };
+          float M = kNegBig, L = 0.f;
+          for (int64_t c = c0; c <= c1; c += P) {
+            float pm[P], pl[P], m_new = M;
+#pragma unroll
+            for (int i = 0; i < P; ++i) {
+              pm[i] = c + i <= c1 ? __ldcg(part_of(c + i)) : kNegBig;
+              pl[i] = c + i <= c1 ? __ldcg(part_of(c + i) + kTileRows) : 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < P; ++i) m_new = fmaxf(m_new, pm[i]);
+            L *= ex2(M - m_new);
+#pragma unroll
+            for (int i = 0; i < P; ++i) L += pl[i] * ex2(pm[i] - m_new);
+            M = m_new;
+          }
+#pragma unroll 1
+          for (int d = d_lo; d < d_hi; d += 16) {
+            float y[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) y[i] = 0.f;
+            for (int64_t c = c0; c <= c1; c += P) {
+              float v[P][16], f[P];
+#pragma unroll
+              for (int k = 0; k < P; ++k) {
+                f[k] = c + k <= c1 ? ex2(__ldcg(part_of(c + k)) - M) : 0.f;
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                  v[k][i] = c + k <= c1 ? __ldcg(part_of(c + k) + (2 + d + i) * kTileRows) : 0.f;
+              }
+#pragma unroll
+              for (int k = 0; k < P; ++k)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) y[i] = fmaf(v[k][i], f[k], y[i]);
+            }
+            put(d, y, 1.f / L, L == 0.f);
+          }
+        }
+      }
+      kc0 += g.nt;
+      // The next job's query rows and statistics take the same places: not
+      // before both groups are done with these.
+      tc_fence_before();
+      named_bar_sync(2, 256);
     }
-    tc_fence_before();
-    __syncthreads();  // shared and tensor memory are reused by the next job
-    tc_fence_after();
-    kc0 += nt;
-    done[0] += (ns + 1) / 2;
-    done[1] += ns / 2;
-    u += k1 - k0;
   }
+  tc_fence_before();
   __syncthreads();
-  if (warp == 12) tmem_dealloc(tmem, 512);
+  tc_fence_after();
+  if (warp == 16) tmem_dealloc(tmem, 512);
 }
 
 template <int D, bool FP8>
 void launch_tiles(const Args& a, cudaStream_t stream) {
-  const int smem = TileSmem<D>::bytes(a.B);
+  const int smem = TileSmem<D, FP8>::bytes(a.B);
   static int configured = 0;
   if (smem > configured) {
     CB_CUDA_CHECK(cudaFuncSetAttribute(attn_tiles_kernel<D, FP8>,
                                        cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    cudaFuncAttributes attr;
+    CB_CUDA_CHECK(cudaFuncGetAttributes(&attr, attn_tiles_kernel<D, FP8>));
+    if (attr.numRegs < kRegsLaunch)  // the groups' shares would never come free
+      throw std::runtime_error("attn_tiles_kernel was built with too few registers a thread");
     configured = smem;
   }
   launch_kernel(attn_tiles_kernel<D, FP8>, dim3(num_sms()), dim3(kTileThreads), smem, stream, a);

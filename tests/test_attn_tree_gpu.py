@@ -244,6 +244,18 @@ def test_extreme_scales(nodes):
 
 
 @pytest.mark.parametrize("cache", ["fp8", "bf16"])
+@pytest.mark.parametrize("nodes", [1, 4, 40])
+def test_values_of_zero(cache, nodes):
+    """A head whose values are all zero (the smallest scale) over a long
+    context, alone and beside ordinary heads."""
+    p = Problem(cache, 8, 2, 128, [9000, 30 + nodes], [nodes, nodes], seed=18,
+                v_mul=lambda shape, g: torch.tensor([0.0, 1.0]).view(1, 2, 1))
+    out = p.run()
+    p.check(out)
+    assert bool((out.view(-1, 2, 4, 128)[:, 0] == 0).all())
+
+
+@pytest.mark.parametrize("cache", ["fp8", "bf16"])
 def test_value_of_one_key_comes_back(cache):
     """A sequence of one key returns its value, to the last bit."""
     p = Problem(cache, 6, 2, 128, [1, 1], [1, 1], tree=False, seed=10)
