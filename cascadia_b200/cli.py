@@ -68,7 +68,9 @@ def _common(p: argparse.ArgumentParser):
     p.add_argument("--tokenizer", default=None)
     p.add_argument("--log-level", default="info")
     p.add_argument("--max-concurrent", type=int, default=16)
-    p.add_argument("--spec", default=None, choices=["ngram", "draft", "mtp"],
+    p.add_argument("--kv-dtype", default=_env("KV_DTYPE", "bf16"), choices=["bf16", "fp8"],
+                   help="KV cache: bf16, or e4m3 codes with a scale per token and head")
+    p.add_argument("--spec", default=None, choices=["ngram", "draft", "mtp", "tree"],
                    help="speculative decoding of greedy requests")
     p.add_argument("--spec-k", type=int, default=4, help="draft tokens per round")
     p.add_argument("--draft-model", default=None, help="draft model preset (--spec draft)")
@@ -107,14 +109,14 @@ def _builder(args, tp=None):
 
         return MoEBuilder(args.model, device=args.device, kv_blocks=args.kv_blocks,
                           max_running=args.max_running, max_model_len=args.max_model_len,
-                          seed=args.seed)
+                          seed=args.seed, kv_dtype=args.kv_dtype)
     return LLMBuilder(args.model, device=args.device, kv_blocks=args.kv_blocks,
                       kv_fraction=args.kv_fraction, max_running=args.max_running,
                       max_model_len=args.max_model_len,
                       prefix_cache_blocks=args.kv_prefix_cache_size,
                       use_graph=not args.no_cuda_graph, seed=args.seed, tp=tp,
                       tokenizer_path=args.tokenizer, spec=args.spec, spec_k=args.spec_k,
-                      draft_model=args.draft_model)
+                      draft_model=args.draft_model, kv_dtype=args.kv_dtype)
 
 
 def validate_run_flags(args) -> None:
@@ -153,6 +155,10 @@ def validate_run_flags(args) -> None:
             "is --engine spec)")
     if args.spec == "draft" and not args.draft_model:
         bad("--spec draft needs --draft-model")
+    if args.spec == "tree" and getattr(args, "tp", 1) > 1:
+        bad("--spec tree runs on one GPU")
+    if getattr(args, "kv_dtype", "bf16") != "bf16" and (pp > 1 or getattr(args, "ep", 1) > 1):
+        bad("--kv-dtype fp8 is served without pipeline stages and expert parallelism")
     if tp > 1 and not os.path.isdir(str(args.model)):
         from .models.config import PRESETS
 

@@ -82,9 +82,17 @@ class LLMEngine(Engine):
         self.pipeline = None
         # Speculative decoding of greedy sequences: "ngram" (prompt lookup),
         # "draft" (a small model with its own KV, ``draft_model``) or "mtp"
-        # (a GLM-5 multi-token-prediction head, ``mtp_head``).
-        if spec not in (None, "ngram", "draft", "mtp"):
+        # (a GLM-5 multi-token-prediction head, ``mtp_head``), or "tree"
+        # (n-gram drafts as a tree, where the text has gone on differently).
+        if spec not in (None, "ngram", "draft", "mtp", "tree"):
             raise InvalidConfig(f"unknown speculative mode {spec!r}")
+        if spec == "tree":
+            if model.tp.size > 1:
+                raise InvalidConfig("speculative mode 'tree' runs on one GPU")
+            try:
+                model.check_new_token_attention("speculative mode 'tree'")
+            except ValueError as e:
+                raise InvalidConfig(str(e)) from e
         if spec == "draft" and draft_model is None:
             raise InvalidConfig("speculative mode 'draft' needs a draft model")
         if spec == "mtp" and (mtp_head is None or pc is not None):
@@ -355,11 +363,53 @@ class LLMEngine(Engine):
         for s, t in zip(seqs, toks):
             self._emit(s, int(t), out, lps.get(s.seq_id))
 
+    def _spec_decode_trees(self, seqs: List[Sequence], out):
+        """One speculative round with n-gram trees; sequences that asked for
+        logprobs take part (the verification computes them)."""
+        from ..runtime.spec import MAX_TREE_NODES, NGramDraft, verify_trees
+
+        m = self.model
+        trees = []
+        for s in seqs:
+            if getattr(s, "ngram", None) is None:
+                s.ngram = NGramDraft(self.spec_k)
+                s.ngram.extend(s.prompt_ids + s.output_ids)
+            room = min(s.task.max_tokens - len(s.output_ids),
+                       self.max_model_len - s.total_len - 1) - 1
+            trees.append(s.ngram.propose_tree(self.spec_k, min(31, MAX_TREE_NODES)).cut(
+                max(0, room)))
+        k = max(min(20, s.task.logprobs) for s in seqs)
+        results = verify_trees(m, [s.seq_id for s in seqs], [s.output_ids[-1] for s in seqs],
+                               trees, [s.total_len - 1 for s in seqs], k)
+        if self._device_failed(seqs, out):
+            return
+        st = self.spec_stats
+        st.rounds += 1
+        metrics.SPEC_PROPOSED.labels(model=self.model_id).inc(sum(len(t.tokens) for t in trees))
+        metrics.SPEC_ACCEPTED.labels(model=self.model_id).inc(
+            sum(len(r.tokens) - 1 for r in results))
+        for s, tree, r in zip(seqs, trees, results):
+            st.drafted += len(tree.tokens)
+            st.accepted += len(r.tokens) - 1
+            st.emitted += len(r.tokens)
+            for t, lp, ids, top in zip(r.tokens, r.logprobs, r.top_ids, r.top_logprobs):
+                info = None
+                if s.task.logprobs > 0:
+                    info = self._token_logprobs(int(t), lp, ids, top, s.task.logprobs)
+                self._emit(s, int(t), out, info)
+                s.ngram.append(int(t))
+                if s.finished:
+                    break
+
     def _spec_decode(self, seqs: List[Sequence], out):
         """One speculative round for greedy sequences: draft, verify in one
         multi-token target forward, emit the accepted tokens + correction,
         rewind the KV to the accepted prefix."""
         from ..runtime.spec import NGramDraft, verify_batch
+
+        if self.spec == "tree":
+            self._spec_decode_trees(seqs, out)
+            return
 
         m = self.model
         k = self.spec_k
@@ -467,8 +517,10 @@ class LLMEngine(Engine):
         return zlib.crc32(s.seq_id.encode()) & 0x7FFFFFFF
 
     def _speculable(self, s: Sequence) -> bool:
-        """Greedy, unpenalised sequences without logprobs decode speculatively."""
-        return s.task.temperature <= 0 and not self._has_penalty(s) and s.task.logprobs <= 0
+        """Greedy, unpenalised sequences without logprobs decode speculatively
+        (trees: with logprobs too)."""
+        return (s.task.temperature <= 0 and not self._has_penalty(s)
+                and (s.task.logprobs <= 0 or self.spec == "tree"))
 
     def _logprobs(self, rows, logits: torch.Tensor, toks) -> Dict[str, TokenLogprobs]:
         """Per-token logprobs for the rows whose task asked for them: the
@@ -481,23 +533,22 @@ class LLMEngine(Engine):
             return {}
         full = self.model.full_logits(logits)
         idx = torch.tensor([i for i, _ in want], dtype=torch.long, device=full.device)
-        lp = torch.log_softmax(full.index_select(0, idx).float(), dim=-1)
         k = max(min(20, s.task.logprobs) for _, s in want)
-        top_v, top_i = lp.topk(k, dim=-1)
-        chosen = torch.tensor([int(toks[i]) for i, _ in want], dtype=torch.long,
+        chosen = torch.tensor([int(toks[i]) for i, _ in want], dtype=torch.int32,
                               device=full.device)
-        ch = lp.gather(1, chosen.unsqueeze(1)).squeeze(1)
+        fn = ops.token_logprobs if full.is_cuda else ref.token_logprobs
+        ch, _, top_i, top_v = fn(full.index_select(0, idx), chosen, k)
         top_v, top_i, ch = top_v.cpu().tolist(), top_i.cpu().tolist(), ch.cpu().tolist()
-        out = {}
-        for r, (i, s) in enumerate(want):
-            n = min(20, s.task.logprobs)
-            tid = int(toks[i])
-            out[s.seq_id] = TokenLogprobs(
-                token=self.tok.decode([tid]), token_id=tid, logprob=float(ch[r]),
-                top_logprobs=[TopLogprob(token=self.tok.decode([int(t)]), token_id=int(t),
-                                         logprob=float(v))
-                              for t, v in zip(top_i[r][:n], top_v[r][:n])])
-        return out
+        return {s.seq_id: self._token_logprobs(int(toks[i]), ch[r], top_i[r], top_v[r],
+                                               s.task.logprobs)
+                for r, (i, s) in enumerate(want)}
+
+    def _token_logprobs(self, tid: int, lp: float, ids, top, count: int) -> TokenLogprobs:
+        n = min(20, count)
+        return TokenLogprobs(
+            token=self.tok.decode([tid]), token_id=tid, logprob=float(lp),
+            top_logprobs=[TopLogprob(token=self.tok.decode([int(t)]), token_id=int(t),
+                                     logprob=float(v)) for t, v in zip(ids[:n], top[:n])])
 
     @staticmethod
     def _has_penalty(s: Sequence) -> bool:
@@ -550,7 +601,8 @@ class LLMBuilder(Builder):
                  prefix_cache_blocks: int = 0, use_graph: bool = True, seed: int = 0,
                  tp=None, tokenizer_path: Optional[str] = None, spec: Optional[str] = None,
                  spec_k: int = 4, draft_model: Optional[str] = None, draft_kv_blocks: int = 0,
-                 ep=None, max_prefill_tokens: int = 8192):
+                 ep=None, max_prefill_tokens: int = 8192, kv_dtype: str = "bf16"):
+        self.kv_dtype = kv_dtype
         self.ep = ep  # parallel.ep.ExpertParallel: this rank's share of the experts
         self.max_prefill_tokens = max_prefill_tokens
         self.spec = spec
@@ -638,11 +690,18 @@ class LLMBuilder(Builder):
         self.tokenizer = load_tokenizer(tok_dir, cfg.vocab_size, cfg.eos_token_ids[0])
         blocks = self.kv_blocks
         hybrid = cfg.is_hybrid
+        kv_args = {}
+        if self.kv_dtype != "bf16":
+            try:
+                self.model.check_new_token_attention(f"--kv-dtype {self.kv_dtype}")
+            except (AttributeError, ValueError) as e:
+                raise InvalidConfig(str(e)) from e
+            kv_args = {"kv_dtype": self.kv_dtype}
         if hybrid and (self.spec or self.prefix_cache_blocks):
             raise InvalidConfig("the linear-attention state of this model cannot be shared or "
                                 "rewound: no prefix cache, no speculative decoding")
         if blocks <= 0:
-            per = self.model.kv_bytes_per_block()
+            per = self.model.kv_bytes_per_block(**kv_args)
             if torch.device(self.device).type == "cuda":
                 free, _ = torch.cuda.mem_get_info(torch.device(self.device))
                 if hybrid:  # recurrent state of every running sequence first
@@ -662,8 +721,8 @@ class LLMBuilder(Builder):
         if hybrid:
             self.model.allocate_kv(blocks, max_seqs=self.max_running)
         else:
-            self.model.allocate_kv(blocks)
-        yield LoadProgress.msg(f"kv cache: {blocks} blocks")
+            self.model.allocate_kv(blocks, **kv_args)
+        yield LoadProgress.msg(f"kv cache: {blocks} blocks ({self.kv_dtype})")
         if self.spec == "draft":
             if not self.draft_name:
                 raise InvalidConfig("--spec draft needs --draft-model")

@@ -124,6 +124,8 @@ class G4MoE:
 
 
 class Gemma4Model(LlamaModel):
+    plain_cache = False
+
     def __init__(self, cfg: ModelConfig, device, tp=None, layer_start: int = 0,
                  layer_end: Optional[int] = None, has_embed: bool = True, has_head: bool = True,
                  **_):

@@ -124,6 +124,10 @@ def random_int4(n: int, k: int, g: torch.Generator, device, std=0.02, group_size
 
 
 class LlamaModel:
+    # Every layer's K / V rows lie in one paged cache with the plain layout:
+    # what drafted trees and the 8-bit cache need.
+    plain_cache = True
+
     def __init__(self, cfg: ModelConfig, device, tp: Optional[TPGroup] = None,
                  layer_start: int = 0, layer_end: Optional[int] = None,
                  has_embed: bool = True, has_head: bool = True):
@@ -298,12 +302,23 @@ class LlamaModel:
         out.copy_(buf)
         return out
 
-    def allocate_kv(self, num_blocks: int) -> KVCache:
-        self.kv = KVCache(self.num_local_layers, num_blocks, self.hkv, self.d, self.device)
+    def allocate_kv(self, num_blocks: int, kv_dtype: str = "bf16") -> KVCache:
+        """``kv_dtype="fp8"``: the 8-bit cache (head_dim 64 or 128, no
+        sliding window)."""
+        if kv_dtype == "fp8":
+            self.check_new_token_attention("the 8-bit KV cache")
+        self.kv = KVCache(self.num_local_layers, num_blocks, self.hkv, self.d, self.device,
+                          kv_dtype=kv_dtype)
         return self.kv
 
-    def kv_bytes_per_block(self) -> int:
-        return KVCache.bytes_per_block(self.num_local_layers, self.hkv, self.d)
+    def check_new_token_attention(self, what: str):
+        """Raise unless ops.attn_tree covers this model's attention."""
+        if not self.plain_cache or self.d not in (64, 128) or self.cfg.sliding_window > 0:
+            raise ValueError(f"{what}: head_dim 64 or 128, no sliding window and one plain paged "
+                             f"cache are needed ({type(self).__name__}, head_dim {self.d})")
+
+    def kv_bytes_per_block(self, kv_dtype: str = "bf16") -> int:
+        return KVCache.bytes_per_block(self.num_local_layers, self.hkv, self.d, kv_dtype=kv_dtype)
 
     # ------------------------------------------------------------ forward
     def embed_tokens(self, ids: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -392,7 +407,7 @@ class LlamaModel:
         the projection's epilogue applies RoPE and writes K / V into the
         paged cache (one launch less per layer)."""
         T = h.shape[0]
-        if (self.device.type == "cuda" and lw.qkv.blob is not None and
+        if (self.device.type == "cuda" and lw.qkv.blob is not None and not self.kv.fp8 and
                 ops.rope_fusable(T, self.d, self.cfg.rot_dim, lw.qkv.group_size)):
             qkv = torch.empty(T, lw.qkv.n, dtype=torch.bfloat16, device=self.device)
             ops.w4a16_gemm_rope_kv(h, lw.qkv.blob, lw.qkv.n, lw.qkv.group_size, qkv,
@@ -407,16 +422,28 @@ class LlamaModel:
         kv = self.kv
         T = qkv.shape[0]
         if self.device.type == "cuda":
-            if not roped:
+            if kv.fp8:
+                ops.rope_kv_write_fp8(qkv, batch.positions, self.cos_sin, batch.slots, kv.k, kv.v,
+                                      kv.k_scale, kv.v_scale, li, hq, hkv, d, self.cfg.rot_dim)
+            elif not roped:
                 ops.rope_kv_write(qkv, batch.positions, self.cos_sin, batch.slots, kv.k, kv.v,
                                   li, hq, hkv, d, self.cfg.rot_dim)
             out = torch.empty(T, hq * d, dtype=torch.bfloat16, device=self.device)
             q = qkv[:, :hq * d]
             win, sinks = self.cfg.sliding_window, self.cfg.attention_sinks
-            if batch.is_decode:
+            if batch.masks is not None or (kv.fp8 and batch.is_decode):
+                ops.attn_tree(q, kv.k, kv.v, batch.block_tables, batch.seq_lens,
+                              batch.rows_of_seqs(), out, li, self.scale, masks=batch.masks,
+                              k_scale=kv.k_scale, v_scale=kv.v_scale, max_nodes=batch.max_nodes)
+            elif batch.is_decode:
                 ops.attn_decode(q, kv.k, kv.v, batch.block_tables, batch.seq_lens, out, li,
                                 batch.num_splits, batch.blocks_per_split, batch.part_o,
                                 batch.part_ml, self.scale, win, sinks)
+            elif kv.fp8:
+                # Prompts: the context's blocks back to bf16 for the prefill kernel.
+                blocks, tables = batch.read_plan()
+                k16, v16 = kv.read_back(li, blocks)
+                ops.attn_prefill(q, k16, v16, tables, batch.tiles, out, 0, self.scale)
             else:
                 ops.attn_prefill(q, kv.k, kv.v, batch.block_tables, batch.tiles, out, li,
                                  self.scale, win, sinks)
@@ -427,18 +454,18 @@ class LlamaModel:
         q = ref.apply_rope(x[:, :hq], pos, self.cos_sin, self.cfg.rot_dim)
         k = ref.apply_rope(x[:, hq:hq + hkv], pos, self.cos_sin, self.cfg.rot_dim)
         v = x[:, hq + hkv:]
-        slots = batch.slots.long()
-        valid = slots >= 0
-        sb, so = slots[valid] // BLOCK_SIZE, slots[valid] % BLOCK_SIZE
-        kv.k[li, sb, :, so] = k[valid].to(torch.bfloat16)
-        kv.v[li, sb, :, so] = v[valid].to(torch.bfloat16)
+        kv.write_rows(li, batch.slots, k, v)
         out = torch.empty(T, hq * d, dtype=torch.float32)
         row = 0
         for sid, ql in zip(batch.seq_ids, batch.q_lens):
             kk, vv = kv.gather(li, sid)
             ctx = int(batch.ctx_len_of(sid))
-            o = ref.attention(q[row:row + ql], kk[:ctx], vv[:ctx], pos[row:row + ql], self.scale,
-                              self.cfg.sliding_window, self.cfg.attention_sinks)
+            if batch.masks is not None:
+                o = ref.tree_attention(q[row:row + ql], kk[:ctx], vv[:ctx], self.scale,
+                                       batch.masks[row:row + ql])
+            else:
+                o = ref.attention(q[row:row + ql], kk[:ctx], vv[:ctx], pos[row:row + ql],
+                                  self.scale, self.cfg.sliding_window, self.cfg.attention_sinks)
             out[row:row + ql] = o.reshape(ql, hq * d)
             row += ql
         return out.to(torch.bfloat16)
@@ -492,6 +519,35 @@ class Batch:
     blocks_per_split: int = 1
     part_o: Optional[torch.Tensor] = None
     part_ml: Optional[torch.Tensor] = None
+    # Drafted trees (runtime.spec.build_tree_batch): the rows each row sees
+    # among its sequence's own, and the largest number of rows of a sequence.
+    masks: Optional[torch.Tensor] = None   # int64 [T]
+    max_nodes: int = 1
+    row_start: Optional[torch.Tensor] = None  # int32 [B + 1]
+    _read: Optional[tuple] = None
+
+    def rows_of_seqs(self) -> torch.Tensor:
+        """First row of every sequence, and the number of rows."""
+        if self.row_start is None:
+            starts = [0]
+            for n in self.q_lens:
+                starts.append(starts[-1] + n)
+            self.row_start = torch.tensor(starts, dtype=torch.int32).to(self.positions.device)
+        return self.row_start
+
+    def read_plan(self):
+        """(all blocks of the sequences' contexts [N], tables of their places
+        in that list): what reading the 8-bit cache back for a prefill needs."""
+        if self._read is None:
+            need = [-(-n // BLOCK_SIZE) for n in self.ctx_lens]
+            blocks = torch.cat([self.block_tables[i, :n] for i, n in enumerate(need)])
+            tables = torch.zeros(len(need), max(need + [1]), dtype=torch.int32)
+            at = 0
+            for i, n in enumerate(need):
+                tables[i, :n] = torch.arange(at, at + n, dtype=torch.int32)
+                at += n
+            self._read = (blocks.contiguous(), tables.to(self.block_tables.device))
+        return self._read
 
     def ctx_len_of(self, sid: str) -> int:
         return self.ctx_lens[self.seq_ids.index(sid)]

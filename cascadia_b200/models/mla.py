@@ -81,6 +81,8 @@ class MLAAttention:
 
 
 class MLAModel(MoEModel):
+    plain_cache = False
+
     def __init__(self, cfg, device, **kw):
         kw.setdefault("bf16_attention", False)
         super().__init__(cfg, device, **kw)

@@ -113,6 +113,8 @@ class HybridLayer(MoELayer):
 
 
 class HybridMoEModel(MoEModel):
+    plain_cache = False
+
     def __init__(self, cfg: ModelConfig, device, tp=None, layer_start: int = 0,
                  layer_end: Optional[int] = None, has_embed: bool = True, has_head: bool = True,
                  ep=None):

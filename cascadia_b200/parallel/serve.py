@@ -171,7 +171,8 @@ def build_tp_engine(args, ctx: DistContext):
                          prefix_cache_blocks=args.kv_prefix_cache_size,
                          use_graph=not args.no_cuda_graph, seed=args.seed, tp=tp,
                          tokenizer_path=args.tokenizer, spec=args.spec, spec_k=args.spec_k,
-                         draft_model=args.draft_model)
+                         draft_model=args.draft_model,
+                         kv_dtype=getattr(args, "kv_dtype", "bf16"))
     if ctx.device.type == "cuda" and ctx.world > 1:
         from .tp import FusedTP
 

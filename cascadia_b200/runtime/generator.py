@@ -143,6 +143,7 @@ class BatchGenerator:
         self.use_graph = use_graph
         self.graphs: Dict[tuple, DecodeGraph] = {}
         self.last_hidden: Optional[torch.Tensor] = None
+        self.last_logits: Optional[torch.Tensor] = None  # of the last prefill or decode step
 
     def prefill(self, seq_ids: Sequence[str], prompts: Sequence[Sequence[int]],
                 start: Optional[Sequence[int]] = None) -> torch.Tensor:
@@ -158,7 +159,7 @@ class BatchGenerator:
         m.forward(batch, hidden)
         self.last_hidden = hidden  # pre-norm rows of every prompt token (MTP drafting)
         last = torch.tensor(batch.last_rows, dtype=torch.long, device=m.device)
-        logits = m.head(hidden.index_select(0, last).contiguous())
+        logits = self.last_logits = m.head(hidden.index_select(0, last).contiguous())
         return m.greedy(logits)
 
     def decode_graph(self, seq_ids: Sequence[str], width: int) -> DecodeGraph:
@@ -195,13 +196,15 @@ class BatchGenerator:
             batch = build_batch(m, seq_ids, [1] * len(seq_ids), starts, decode=True)
             hidden = m.embed_tokens(torch.tensor(list(last_tokens), dtype=torch.int32))
             m.forward(batch, hidden)
-            return m.greedy(m.head(hidden))
+            self.last_logits = m.head(hidden)
+            return m.greedy(self.last_logits)
         g = self.decode_graph(seq_ids, width)
         self.stage_decode_inputs(g, seq_ids, last_tokens)
         g.upload()
         if g.use_graph and g.graph is None:
             g.capture()
         g.run()
+        self.last_logits = g.logits
         return g.download()
 
     def generate(self, prompts: Sequence[Sequence[int]], max_new_tokens: int,

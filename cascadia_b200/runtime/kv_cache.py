@@ -6,7 +6,10 @@ and the geometric-grow bf16 buffers of crates/cascadia-engine-sparse-moe/src/run
 with one device pool addressed through per-sequence block tables.
 
 Storage layout: ``[num_layers, num_blocks, kv_heads, 16, head_dim]`` for K and
-for V, so that one (layer, block, head) tile is contiguous for TMA.
+for V, so that one (layer, block, head) tile is contiguous for TMA.  With
+``kv_dtype="fp8"`` K and V are e4m3 codes of that layout with one fp32 scale per
+(token, kv head), ``[num_layers, num_blocks, kv_heads, 16]``: head_dim + 4 bytes a
+row instead of 2 head_dim.
 """
 from __future__ import annotations
 
@@ -16,6 +19,7 @@ from typing import Dict, List, Optional
 import torch
 
 BLOCK_SIZE = 16
+KV_DTYPES = ("bf16", "fp8")
 
 
 class BlockAllocator:
@@ -54,6 +58,11 @@ class BlockAllocator:
         return self._ref[b]
 
 
+def _bytes(pool: torch.Tensor) -> torch.Tensor:
+    """8-bit pools as bytes (indexing is not defined for float8 tensors)."""
+    return pool.view(torch.uint8) if pool.element_size() == 1 else pool
+
+
 @dataclass
 class SeqKV:
     """Block table and length of one sequence."""
@@ -68,8 +77,15 @@ class SeqKV:
 class KVCache:
     """Device K/V pools for the layers held by this rank."""
 
+    fp8 = False
+    k_scale = v_scale = None
+
     def __init__(self, num_layers: int, num_blocks: int, kv_heads: int, head_dim: int,
-                 device, dtype=torch.bfloat16, v_head_dim: Optional[int] = None):
+                 device, dtype=torch.bfloat16, v_head_dim: Optional[int] = None,
+                 kv_dtype: str = "bf16"):
+        if kv_dtype not in KV_DTYPES:
+            raise ValueError(f"unknown KV cache type {kv_dtype!r} (one of {KV_DTYPES})")
+        self.fp8 = kv_dtype == "fp8"
         self.num_layers = num_layers
         self.num_blocks = num_blocks
         self.kv_heads = kv_heads
@@ -77,15 +93,27 @@ class KVCache:
         shape = (num_layers, num_blocks, kv_heads, BLOCK_SIZE, head_dim)
         # Zero-init: kernels read whole 16-token blocks, so never-written
         # slots must hold finite values.
-        self.k = torch.zeros(shape, dtype=dtype, device=device)
         vshape = (num_layers, num_blocks, kv_heads, BLOCK_SIZE, v_head_dim or head_dim)
-        self.v = torch.zeros(vshape, dtype=dtype, device=device)
+        if self.fp8:
+            self.k = torch.zeros(shape, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn)
+            self.v = torch.zeros(vshape, dtype=torch.uint8, device=device).view(
+                torch.float8_e4m3fn)
+            self.k_scale = torch.ones(shape[:4], dtype=torch.float32, device=device)
+            self.v_scale = torch.ones(shape[:4], dtype=torch.float32, device=device)
+        else:
+            self.k = torch.zeros(shape, dtype=dtype, device=device)
+            self.v = torch.zeros(vshape, dtype=dtype, device=device)
+        # bf16 copies of one layer's blocks that the prefill attention reads
+        # (8-bit cache only): grown as needed, reused by every layer.
+        self._staging = None
         self.allocator = BlockAllocator(num_blocks)
         self.seqs: Dict[str, SeqKV] = {}
 
     @staticmethod
-    def bytes_per_block(num_layers, kv_heads, head_dim, dtype_bytes=2) -> int:
-        return 2 * num_layers * kv_heads * BLOCK_SIZE * head_dim * dtype_bytes
+    def bytes_per_block(num_layers, kv_heads, head_dim, dtype_bytes=2,
+                        kv_dtype: str = "bf16") -> int:
+        row = head_dim + 4 if kv_dtype == "fp8" else head_dim * dtype_bytes
+        return 2 * num_layers * kv_heads * BLOCK_SIZE * row
 
     # ------------------------------------------------------------ sequences
     def add_sequence(self, seq_id: str, shared_prefix: Optional[List[int]] = None) -> SeqKV:
@@ -157,6 +185,57 @@ class KVCache:
         """Dense [len, H, D] copies of one sequence's K/V (CPU oracle path)."""
         s = self.seqs[seq_id]
         ids = torch.tensor(s.blocks, dtype=torch.long, device=self.k.device).clamp_min(0)
-        k = self.k[layer, ids].permute(0, 2, 1, 3).reshape(-1, self.kv_heads, self.k.shape[-1])
-        v = self.v[layer, ids].permute(0, 2, 1, 3).reshape(-1, self.kv_heads, self.v.shape[-1])
-        return k, v
+        out = []
+        for pool, scale in ((self.k, self.k_scale), (self.v, self.v_scale)):
+            x = _bytes(pool)[layer, ids].view(pool.dtype)
+            if scale is not None:
+                x = x.float() * scale[layer, ids].unsqueeze(-1)
+            out.append(x.permute(0, 2, 1, 3).reshape(-1, self.kv_heads, pool.shape[-1]))
+        return tuple(out)
+
+    def write_rows(self, layer: int, slots: torch.Tensor, k: torch.Tensor, v: torch.Tensor):
+        """Store token rows [T, H, D] (CPU oracle path), quantised for the
+        8-bit cache; rows whose slot is negative are left out."""
+        from ..ops import reference as ref
+
+        valid = slots >= 0
+        at = (layer, slots[valid].long() // BLOCK_SIZE, slice(None),
+              slots[valid].long() % BLOCK_SIZE)
+        for pool, scale, x in ((self.k, self.k_scale, k), (self.v, self.v_scale, v)):
+            if scale is None:
+                pool[at] = x[valid].to(pool.dtype)
+                continue
+            codes, s = ref.quantise_rows(x[valid])
+            _bytes(pool)[at] = _bytes(codes)
+            scale[at] = s
+
+    def move_rows(self, seq_id: str, src: List[int], dst: List[int]):
+        """Copy the K / V of positions ``src`` of a sequence to positions
+        ``dst``, in every layer (all are read before any is written): a
+        drafted tree's accepted path closes ranks."""
+        pairs = [(a, b) for a, b in zip(src, dst) if a != b]
+        if not pairs:
+            return
+        blocks = self.seqs[seq_id].blocks
+        at = [[blocks[p[i] // BLOCK_SIZE] * BLOCK_SIZE + p[i] % BLOCK_SIZE for p in pairs]
+              for i in (0, 1)]
+        sl = torch.tensor(at, dtype=torch.long).to(self.k.device)
+        (sb, so), (db, do) = (((x // BLOCK_SIZE), (x % BLOCK_SIZE)) for x in sl)
+        for pool in (_bytes(self.k), _bytes(self.v), self.k_scale, self.v_scale):
+            if pool is not None:
+                pool[:, db, :, do] = pool[:, sb, :, so]
+
+    def read_back(self, layer: int, blocks: torch.Tensor):
+        """bf16 copies of ``blocks`` (int32 [N]) of one layer of the 8-bit
+        cache, as pools [1, N, H, 16, D] of their own; valid until the next
+        call."""
+        from .. import ops
+
+        n = blocks.numel()
+        if self._staging is None or self._staging[0].shape[1] < n:
+            shape = (1, n) + tuple(self.k.shape[2:])
+            self._staging = tuple(torch.empty(shape, dtype=torch.bfloat16, device=self.k.device)
+                                  for _ in range(2))
+        ops.kv_read_fp8(self.k, self.v, self.k_scale, self.v_scale, blocks, layer,
+                        self._staging[0], self._staging[1])
+        return self._staging

@@ -86,6 +86,94 @@ class NGramDraft:
             buf.append(t)
         return out
 
+    def propose_tree(self, k: int, max_nodes: int) -> "DraftTree":
+        """Chains that start from what followed the last 4, 3 and 2 tokens
+        (different places of the text may have gone on differently), longest
+        match first, merged where they agree."""
+        tail = self.history[-MAX_NGRAM:]
+        chains = []
+        for n in range(min(MAX_NGRAM, len(tail)), MIN_NGRAM - 1, -1):
+            t = self.table.get(tuple(tail[-n:]))
+            if t is None:
+                continue
+            buf, chain = tail + [t], [t]
+            while len(chain) < k:
+                t = self._next(buf)
+                if t is None:
+                    break
+                chain.append(t)
+                buf.append(t)
+            chains.append(chain)
+        return DraftTree.from_chains(chains, max_nodes)
+
+
+@dataclass
+class DraftTree:
+    """Drafted continuations of one sequence.  Node 0 is the pending token;
+    node i >= 1 holds ``tokens[i - 1]`` after node ``parents[i - 1]`` < i."""
+    tokens: List[int] = field(default_factory=list)
+    parents: List[int] = field(default_factory=list)
+
+    @staticmethod
+    def from_chains(chains: Sequence[Sequence[int]], max_nodes: int) -> "DraftTree":
+        """The trie of the chains, at most ``max_nodes`` nodes; earlier chains
+        first."""
+        t = DraftTree()
+        for chain in chains:
+            at = 0
+            for tok in chain:
+                nxt = t.child(at, tok)
+                if nxt is None:
+                    if len(t.tokens) >= max_nodes:
+                        break
+                    nxt = t.add(at, tok)
+                at = nxt
+        return t
+
+    def add(self, parent: int, token: int) -> int:
+        self.tokens.append(int(token))
+        self.parents.append(parent)
+        return len(self.tokens)
+
+    def child(self, node: int, token: int) -> Optional[int]:
+        for i, (p, t) in enumerate(zip(self.parents, self.tokens)):
+            if p == node and t == token:
+                return i + 1
+        return None
+
+    def depths(self) -> List[int]:
+        d = [0]
+        for p in self.parents:
+            d.append(d[p] + 1)
+        return d
+
+    def masks(self) -> List[int]:
+        """Bit j of entry i: node i sees node j (itself and its ancestors), as
+        signed 64-bit numbers."""
+        m = [1]
+        for i, p in enumerate(self.parents):
+            m.append(m[p] | 1 << (i + 1))
+        return [x - (1 << 64) if x >= 1 << 63 else x for x in m]
+
+    def accepted_chain(self, tokens: Sequence[int]) -> int:
+        """How many of the accepted ``tokens`` follow the first branch at every
+        node (the chain a draft model's own cache holds)."""
+        node = n = 0
+        for tok in tokens:
+            first = next((i + 1 for i, p in enumerate(self.parents) if p == node), None)
+            if first is None or self.tokens[first - 1] != tok:
+                break
+            node, n = first, n + 1
+        return n
+
+    def cut(self, max_depth: int) -> "DraftTree":
+        """Without the nodes deeper than ``max_depth``."""
+        keep, new = {0: 0}, DraftTree()
+        for i, (d, p, t) in enumerate(zip(self.depths()[1:], self.parents, self.tokens)):
+            if d <= max_depth:
+                keep[i + 1] = new.add(keep[p], t)
+        return new
+
 
 def count_accepted(drafts: Sequence[int], target: Sequence[int]) -> int:
     """Length of the longest prefix where the draft equals the target's pick."""
@@ -300,6 +388,108 @@ def verify_batch(m, seq_ids: List[str], pending: List[int], drafts: List[List[in
     return [ref.spec_verify(t[i].tolist(), drafts[i]) for i in range(B)]
 
 
+MAX_TREE_NODES = 63  # of a tree, beside its pending token: one bit each in a 64-bit mask
+
+
+@dataclass
+class TreeResult:
+    """What one sequence's tree came to."""
+    tokens: List[int]            # accepted drafts, then the target's own next token
+    logprobs: List[float]        # the target's log-probability of each
+    entropies: List[float]       # of the distribution each was taken from
+    top_ids: List[List[int]]     # its most likely tokens, with their
+    top_logprobs: List[List[float]]  # log-probabilities
+    draft_logprob: float         # mean log-probability the target gave first drafts
+
+
+def build_tree_batch(m, seq_ids: Sequence[str], trees: Sequence[DraftTree],
+                     kv_lens: Sequence[int]):
+    """The inputs of one forward over every sequence's pending token and
+    drafted nodes: node i of a sequence lies in slot ``kv_len + i`` and is
+    rotated for position ``kv_len + depth``."""
+    from ..models.llama import Batch
+
+    kv, dev = m.kv, m.device
+    pos, slots, ctx, masks, counts = [], [], [], [], []
+    for sid, tree, p0 in zip(seq_ids, trees, kv_lens):
+        n = 1 + len(tree.tokens)
+        kv.reserve(sid, p0 + n)
+        st = kv.seqs[sid]
+        st.length = max(st.length, p0 + n)
+        pos.extend(p0 + d for d in tree.depths())
+        slots.extend(st.slots(p0, p0 + n))
+        masks.extend(tree.masks())
+        ctx.append(p0 + n)
+        counts.append(n)
+    width = max(len(kv.seqs[s].blocks) for s in seq_ids)
+    return Batch(seq_ids=list(seq_ids), q_lens=counts, ctx_lens=ctx,
+                 positions=torch.tensor(pos, dtype=torch.int32).to(dev),
+                 slots=torch.tensor(slots, dtype=torch.int32).to(dev),
+                 block_tables=kv.block_table(list(seq_ids), width, dev),
+                 seq_lens=torch.tensor(ctx, dtype=torch.int32).to(dev), is_decode=False,
+                 masks=torch.tensor(masks, dtype=torch.int64).to(dev), max_nodes=max(counts))
+
+
+def verify_trees(m, seq_ids: Sequence[str], pending: Sequence[int], trees: Sequence[DraftTree],
+                 kv_lens: Sequence[int], top_k: int = 1) -> List[TreeResult]:
+    """One target forward over all trees; per sequence the longest path of
+    drafts that greedy decoding would have taken, and the token after it.
+    The accepted path's K / V rows are moved together and the cache is cut
+    after them, so the caller goes on from ``kv_len + len(tokens)``.  Single
+    GPU or CPU, models with a plain paged cache."""
+    m.check_new_token_attention("drafted trees")
+    if m.tp.size > 1:
+        raise ValueError("drafted trees are verified on one GPU")
+    if any(len(t.tokens) > MAX_TREE_NODES for t in trees):
+        raise ValueError(f"a tree has at most {MAX_TREE_NODES} drafted nodes")
+    batch = build_tree_batch(m, seq_ids, trees, kv_lens)
+    flat = [t for p, tree in zip(pending, trees) for t in [p] + tree.tokens]
+    hidden = m.embed_tokens(torch.tensor(flat, dtype=torch.int32).to(m.device))
+    m.forward(batch, hidden)
+    logits = m.head(hidden)[:, :m.vocab_valid]
+    # The draft each node was followed by first: what the target thinks of it.
+    first = []
+    for tree in trees:
+        follow = [-1] * (1 + len(tree.tokens))
+        for t, p in zip(reversed(tree.tokens), reversed(tree.parents)):
+            follow[p] = t
+        first.extend(follow)
+    given = torch.tensor(first, dtype=torch.int32).to(m.device)
+    k = max(1, top_k)
+    if m.device.type == "cuda":
+        lp, ent, ids, top = ops.token_logprobs(logits, given, k)
+    else:
+        from ..ops import reference as ref
+
+        lp, ent, ids, top = ref.token_logprobs(logits, given, k)
+    ids = ids.cpu().tolist()
+    num = torch.cat([lp[:, None], ent[:, None], top], dim=1).cpu().tolist()
+    out, row = [], 0
+    for sid, tree, p0 in zip(seq_ids, trees, kv_lens):
+        node, path = 0, [0]
+        r = TreeResult([], [], [], [], [], float("nan"))
+        given_lp = [num[row + i][0] for i in range(1 + len(tree.tokens)) if first[row + i] >= 0]
+        if given_lp:
+            r.draft_logprob = sum(given_lp) / len(given_lp)
+        while True:
+            pick = ids[row + node][0]
+            r.tokens.append(pick)
+            r.logprobs.append(num[row + node][2])
+            r.entropies.append(num[row + node][1])
+            r.top_ids.append(ids[row + node])
+            r.top_logprobs.append(num[row + node][2:])
+            nxt = tree.child(node, pick)
+            if nxt is None:
+                break
+            node = nxt
+            path.append(node)
+        m.kv.move_rows(sid, [p0 + i for i in path], list(range(p0, p0 + len(path))))
+        m.kv.truncate(sid, p0 + len(path))
+        out.append(r)
+        row += 1 + len(tree.tokens)
+    return out
+
+
 class ModelDrafter:
     """Greedy drafts from a small model with its own paged KV.  Per sequence
     it remembers how many history tokens its KV holds; a round first feeds
@@ -341,6 +531,47 @@ class ModelDrafter:
             for x, t in zip(drafts, last):
                 x.append(t)
         return drafts
+
+    def propose_trees(self, seq_ids: List[str], histories: List[List[int]], k: int, width: int,
+                      branch: int, max_nodes: int) -> List[DraftTree]:
+        """The greedy chain of ``k`` drafts and, at every depth, the ``branch
+        - 1`` next most likely tokens beside it."""
+        d = self.model
+        cuda = d.device.type == "cuda"
+        tails = []
+        for sid, h in zip(seq_ids, histories):
+            if sid not in d.kv.seqs:
+                d.kv.add_sequence(sid)
+                self.kv_len[sid] = 0
+            tails.append(h[self.kv_len[sid]:])
+        trees = [DraftTree() for _ in seq_ids]
+        at = [0] * len(seq_ids)
+        last = None
+        for step in range(k):
+            if step == 0 and not all(len(t) == 1 for t in tails):
+                self.gen.prefill(seq_ids, tails, [self.kv_len[s] for s in seq_ids])
+            else:
+                self.gen.decode(seq_ids, [t[0] for t in tails] if step == 0 else last, width)
+            logits = self.gen.last_logits[:len(seq_ids), :d.vocab_valid]
+            none = torch.full((len(seq_ids),), -1, dtype=torch.int32, device=logits.device)
+            if cuda:
+                ids = ops.token_logprobs(logits, none, branch)[2]
+            else:
+                from ..ops import reference as ref
+
+                ids = ref.token_logprobs(logits, none, branch)[2]
+            ids = ids.cpu().tolist()
+            if step == 0:
+                for sid, h in zip(seq_ids, histories):
+                    self.kv_len[sid] = len(h)
+            for i, (tree, top) in enumerate(zip(trees, ids)):
+                if len(tree.tokens) + branch <= max_nodes:
+                    node = tree.add(at[i], top[0])
+                    for t in top[1:]:
+                        tree.add(at[i], t)
+                    at[i] = node
+            last = [top[0] for top in ids]
+        return trees
 
     def accept(self, sid: str, accepted: int, k: int):
         """After verify: the draft forwarded d1 .. d_{k-1}; keep the accepted
@@ -540,4 +771,93 @@ class SpecDecoder:
             m.kv.free_sequence(s.sid)
             if self.drafter is not None:
                 self.drafter.release(s.sid)
+        return out
+
+
+class TreeSpecDecoder:
+    """Batched greedy speculative decoding of ``target`` with drafted trees:
+    from a draft model (``draft``: its greedy chain with ``branch - 1``
+    alternatives at every depth) or from the text itself (n-grams that went
+    on differently).  Works on the bf16 and the 8-bit KV cache.  The output
+    equals plain greedy decoding of the target."""
+
+    def __init__(self, target, draft=None, k: int = 4, branch: int = 3, max_nodes: int = 31,
+                 use_graph: bool = True):
+        from .generator import BatchGenerator
+
+        target.check_new_token_attention("drafted trees")
+        if not 1 <= max_nodes <= MAX_TREE_NODES:
+            raise ValueError(f"a tree has 1 to {MAX_TREE_NODES} drafted nodes")
+        self.target, self.k, self.branch, self.max_nodes = target, k, branch, max_nodes
+        self.tgen = BatchGenerator(target, use_graph=use_graph)
+        self.drafter = ModelDrafter(draft, use_graph) if draft is not None else None
+        self.stats = SpecStats()
+
+    def generate(self, prompts: Sequence[Sequence[int]], max_new_tokens: int,
+                 eos: Sequence[int] = (), prefix: str = "tree",
+                 logprobs: Optional[list] = None) -> List[List[int]]:
+        """Generated tokens of every prompt.  ``logprobs``, when given,
+        receives per prompt the log-probability of each token after the first
+        (which the prefill picks)."""
+        m = self.target
+        ids = [f"{prefix}{i}" for i in range(len(prompts))]
+        longest = max(len(p) for p in prompts) + max_new_tokens + self.k + 2
+        width = -(-longest // BLOCK_SIZE)
+        first = self.tgen.prefill(ids, prompts).cpu().tolist()
+        states = []
+        for sid, p, t in zip(ids, prompts, first):
+            s = SpecState(sid, list(p) + [int(t)], kv_len=len(p), generated=1)
+            if self.drafter is None:
+                s.ngram = NGramDraft(self.k)
+                s.ngram.extend(s.tokens)
+            s.done = max_new_tokens <= 1 or int(t) in eos
+            states.append(s)
+        lps = [[] for _ in prompts]
+        while True:
+            live = [(i, s) for i, s in enumerate(states) if not s.done]
+            if not live:
+                break
+            t0 = time.perf_counter()
+            if self.drafter is not None:
+                trees = self.drafter.propose_trees([s.sid for _, s in live],
+                                                   [s.tokens for _, s in live], self.k, width,
+                                                   self.branch, self.max_nodes)
+            else:
+                trees = [s.ngram.propose_tree(self.k, self.max_nodes) for _, s in live]
+            # Never draft past the token budget.
+            trees = [t.cut(max(0, max_new_tokens - s.generated - 1))
+                     for (_, s), t in zip(live, trees)]
+            t1 = time.perf_counter()
+            results = verify_trees(m, [s.sid for _, s in live], [s.tokens[-1] for _, s in live],
+                                   trees, [s.kv_len for _, s in live])
+            self.stats.draft_s += t1 - t0
+            self.stats.verify_s += time.perf_counter() - t1
+            self.stats.rounds += 1
+            for (i, s), tree, r in zip(live, trees, results):
+                a = len(r.tokens) - 1
+                self.stats.drafted += len(tree.tokens)
+                self.stats.accepted += a
+                s.kv_len += 1 + a
+                if self.drafter is not None:
+                    self.drafter.accept(s.sid, tree.accepted_chain(r.tokens[:a]), self.k)
+                new = r.tokens[:max_new_tokens - s.generated]
+                for j, t in enumerate(new):
+                    if t in eos:
+                        new = new[:j + 1]
+                        break
+                s.tokens.extend(new)
+                if s.ngram is not None:
+                    s.ngram.extend(new)
+                s.generated += len(new)
+                self.stats.emitted += len(new)
+                lps[i].extend(r.logprobs[:len(new)])
+                s.done = s.generated >= max_new_tokens or (bool(new) and new[-1] in eos)
+        out = []
+        for s, p in zip(states, prompts):
+            out.append(s.tokens[len(p):])
+            m.kv.free_sequence(s.sid)
+            if self.drafter is not None:
+                self.drafter.release(s.sid)
+        if logprobs is not None:
+            logprobs.extend(lps)
         return out
