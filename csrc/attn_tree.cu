@@ -13,10 +13,12 @@
 //   w_j = 2^(t_j - M),   out = sum_j w_j vc_j / sum_j (w_j / vs_j)
 //
 // so that the weights of the value codes stay in [0, 1] whatever the scales
-// are, for one exponential a score.  e4m3 codes are exact in fp16; q is brought
-// into fp16's range by a power of two of its own for every row, and the weights
-// are held as 2^8 w in fp16 (11 bits; w / vs summed over 2^19 keys stays finite
-// down to the smallest scale, 2^-100).  With the bf16 cache the weights are
+// are, for one exponential a score.  Scores are 8-bit products: the codes of K as
+// they are and q as two e4m3 numbers, q = hi + lo, scaled by a power of two of its
+// own for every row: exact down to 2^-9 of the row's largest value, and to 2^-18 of
+// it below that.  The codes of V are exact in fp16, and the weights are held as
+// 2^8 w in fp16 (11 bits; w / vs summed over 2^19 keys stays finite down to the
+// smallest scale, 2^-100).  With the bf16 cache the weights are
 // rounded to bf16, as its values are.  Sums and statistics are fp32.
 //
 // Work split: the keys of all (sequence, kv head, row tile) jobs form one line
@@ -44,6 +46,15 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], u
                                         uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void mma_e4m3(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
       "{%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -138,13 +149,15 @@ struct Warp {
       const uint32_t w0[4] = {x.k[0][c].x, x.k[0][c].y, x.k[0][c].z, x.k[0][c].w};
       const uint32_t w1[4] = {x.k[1][c].x, x.k[1][c].y, x.k[1][c].z, x.k[1][c].w};
       if constexpr (FP8) {
+        // The codes as they are, times the high and the low parts of q.
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint32_t kf[4];
-          e4m3_to_f16(w0[i], kf[0], kf[2]);
-          e4m3_to_f16(w1[i], kf[1], kf[3]);
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t kf[4] = {w0[2 * i], w1[2 * i], w0[2 * i + 1], w1[2 * i + 1]};
 #pragma unroll
-          for (int n = 0; n < NR; ++n) mma_f16(sc[n], kf, q[n][4 * c + i][0], q[n][4 * c + i][1]);
+          for (int n = 0; n < NR; ++n) {
+            mma_e4m3(sc[n], kf, q[n][4 * c + 2 * i][0], q[n][4 * c + 2 * i + 1][0]);
+            mma_e4m3(sc[n], kf, q[n][4 * c + 2 * i][1], q[n][4 * c + 2 * i + 1][1]);
+          }
         }
       } else {
 #pragma unroll
@@ -350,7 +363,8 @@ __global__ void __launch_bounds__(128, NR == 1 && FP8 ? 3 : 2) attn_rows_kernel(
     Warp<D, FP8, NR> w;
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
-      // Row 8 n + g as the second operand: dims in the K chunks' order.
+      // Row 8 n + g as the second operand: dims in the K chunks' order (8-bit: the
+      // four of a k-step's first 16-bit pair and second in one word).
       const int r = 8 * n + g;
       const bool live = r < rows_left;
       const int rr = tile * ROWS + (live ? r : 0);
@@ -371,22 +385,14 @@ __global__ void __launch_bounds__(128, NR == 1 && FP8 ? 3 : 2) attn_rows_kernel(
       }
       float back = a.scale_log2;
       if constexpr (FP8) {
-        // A power of two that puts the row's largest value into [2^14, 2^15):
-        // what it moves below fp16's smallest value is under 2^-38 of that.
+        // Four dims as e4m3, a high and a low part.
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const int e = (int)(top >> 7);  // biased exponent
-        const int sh = e == 0 || e == 255 ? 0 : min(100, 127 + 14 - e);
-        const float up = __int_as_float((127 + sh) << 23);
-        back *= __int_as_float((127 + 8 - sh) << 23);  // (keys are unpacked times 2^-8)
-        // Dims 0, 2 and 1, 3 of every four, as the keys' codes are unpacked.
+        const QScale qs = q_scale(top);
+        back *= qs.down;
 #pragma unroll
-        for (int ks = 0; ks < NKS; ++ks) {
-          const uint32_t lo = w.q[n][ks][0], hi = w.q[n][ks][1];
-          w.q[n][ks][0] = pack_f16(__uint_as_float(lo << 16) * up, __uint_as_float(hi << 16) * up);
-          w.q[n][ks][1] = pack_f16(__uint_as_float(lo & 0xffff0000u) * up,
-                                   __uint_as_float(hi & 0xffff0000u) * up);
-        }
+        for (int ks = 0; ks < NKS; ++ks)
+          split_e4m3(w.q[n][ks][0], w.q[n][ks][1], qs.up, w.q[n][ks][0], w.q[n][ks][1]);
       }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {

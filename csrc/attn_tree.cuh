@@ -57,6 +57,44 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
+// The power of two that puts a query row's largest value into [2^7, 2^8), from the
+// bits of its largest bf16 magnitude, and the way back.  A row with an infinity or
+// a NaN gets NaN scores.
+struct QScale {
+  float up, down;
+};
+__device__ __forceinline__ QScale q_scale(uint32_t top) {
+  const int e = (int)(top >> 7);
+  const int sh = e == 0 || e == 255 ? 0 : min(100, 127 + 7 - e);
+  QScale s;
+  s.up = __int_as_float((127 + sh) << 23);
+  s.down = e == 255 ? __int_as_float(0x7fc00000) : __int_as_float((127 - sh) << 23);
+  return s;
+}
+
+// Four bf16 values (two words) times `up` as e4m3 numbers: hi + lo has all eight
+// bits of a value that is at least 2^-9 of the row's largest, and is within 2^-18
+// of the largest otherwise.
+__device__ __forceinline__ void split_e4m3(uint32_t a0, uint32_t a1, float up, uint32_t& hi,
+                                           uint32_t& lo) {
+  const float x[4] = {__uint_as_float(a0 << 16) * up, __uint_as_float(a0 & 0xffff0000u) * up,
+                      __uint_as_float(a1 << 16) * up, __uint_as_float(a1 & 0xffff0000u) * up};
+  uint32_t h = 0u, l = 0u;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const uint32_t h8 = __nv_cvt_float2_to_fp8x2(make_float2(x[2 * k], x[2 * k + 1]),
+                                                 __NV_SATFINITE, __NV_E4M3);
+    const float2 back =
+        __half22float2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)h8, __NV_E4M3));
+    const uint32_t l8 = __nv_cvt_float2_to_fp8x2(
+        make_float2(x[2 * k] - back.x, x[2 * k + 1] - back.y), __NV_SATFINITE, __NV_E4M3);
+    h |= h8 << (16 * k);
+    l |= l8 << (16 * k);
+  }
+  hi = h;
+  lo = l;
+}
+
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

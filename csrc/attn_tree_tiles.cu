@@ -648,7 +648,6 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tiles_kernel(const Args 
             smem_u32(smem + S::kQ) + (g.mt == 2 ? wg : 0) * S::kQTile + (tid & 127) * 128;
         const int r = tid & 7;
         if constexpr (FP8) {
-          // A power of two that puts the row's largest value into [2^7, 2^8).
 #pragma unroll
           for (int c = 0; c < D / 8; ++c) {
             const uint32_t w[4] = {y[c].x, y[c].y, y[c].z, y[c].w};
@@ -656,36 +655,15 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tiles_kernel(const Args 
             for (int i = 0; i < 4; ++i)
               top = max(top, max(w[i] & 0x7fffu, (w[i] >> 16) & 0x7fffu));
           }
-          const int e = (int)(top >> 7);
-          const int sh = e == 0 || e == 255 ? 0 : min(100, 127 + 7 - e);
-          const float up = __int_as_float((127 + sh) << 23);
-          row_scale *= __int_as_float((127 - sh) << 23);
-          if (e == 255) row_scale = __int_as_float(0x7fc00000);  // an infinity or a NaN in the row
+          const QScale qs = q_scale(top);
+          row_scale *= qs.down;
 #pragma unroll
           for (int c = 0; c < D / 8; c += 2) {
             uint32_t hi[4], lo[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {  // 4 dims a word
-              const uint4& z = y[c + (i >> 1)];
-              const uint32_t a0 = i & 1 ? z.z : z.x, a1 = i & 1 ? z.w : z.y;
-              const float x[4] = {__uint_as_float(a0 << 16) * up,
-                                  __uint_as_float(a0 & 0xffff0000u) * up,
-                                  __uint_as_float(a1 << 16) * up,
-                                  __uint_as_float(a1 & 0xffff0000u) * up};
-              hi[i] = lo[i] = 0u;
-#pragma unroll
-              for (int k = 0; k < 2; ++k) {
-                const uint32_t h8 = __nv_cvt_float2_to_fp8x2(make_float2(x[2 * k], x[2 * k + 1]),
-                                                             __NV_SATFINITE, __NV_E4M3);
-                const float2 back = __half22float2(
-                    __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)h8, __NV_E4M3));
-                const uint32_t l8 = __nv_cvt_float2_to_fp8x2(
-                    make_float2(x[2 * k] - back.x, x[2 * k + 1] - back.y), __NV_SATFINITE,
-                    __NV_E4M3);
-                hi[i] |= h8 << (16 * k);
-                lo[i] |= l8 << (16 * k);
-              }
-            }
+            split_e4m3(y[c].x, y[c].y, qs.up, hi[0], lo[0]);
+            split_e4m3(y[c].z, y[c].w, qs.up, hi[1], lo[1]);
+            split_e4m3(y[c + 1].x, y[c + 1].y, qs.up, hi[2], lo[2]);
+            split_e4m3(y[c + 1].z, y[c + 1].w, qs.up, hi[3], lo[3]);
             if (writes) {
               const uint32_t at = dst + (((c >> 1) ^ r) << 4);
               sts128(at, hi[0], hi[1], hi[2], hi[3]);
