@@ -109,13 +109,6 @@ __device__ __forceinline__ uint4 ldg_stream16(const void* p) {
                : "l"(p));
   return v;
 }
-__device__ __forceinline__ uint2 ldg_stream8(const void* p) {
-  uint2 v;
-  asm("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];"
-               : "=r"(v.x), "=r"(v.y)
-               : "l"(p));
-  return v;
-}
 
 // n rows, len keys in nb units of UNIT tokens (one at least), read by `tiles`
 // row tiles.
@@ -133,9 +126,11 @@ __device__ __forceinline__ SeqShape seq_shape(const Args& a, int b, int rows) {
   return s;
 }
 
-// pre[b] = units of work before sequence b; pre[B] = all of it.
+// pre[b] = units of work of `heads` kv heads before sequence b; pre[B] = all of it.
+// seqs[b], if asked for: its keys and first row; seqs[B].y: the end of the rows.
 template <int UNIT, int THREADS>
-__device__ __forceinline__ void scan_work(const Args& a, int rows, int64_t* pre, int64_t* warp_sum) {
+__device__ __forceinline__ void scan_work(const Args& a, int rows, int heads, int64_t* pre,
+                                          int64_t* warp_sum, int2* seqs = nullptr) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int64_t carry = 0;
   if (tid == 0) pre[0] = 0;
@@ -144,7 +139,12 @@ __device__ __forceinline__ void scan_work(const Args& a, int rows, int64_t* pre,
     int64_t u = 0;
     if (b < a.B) {
       const SeqShape s = seq_shape<UNIT>(a, b, rows);
-      u = (int64_t)a.Hkv * s.tiles * s.nb;
+      u = (int64_t)heads * s.tiles * s.nb;
+      if (seqs != nullptr) {
+        const int row0 = a.row_start[b];
+        seqs[b] = make_int2(s.len, row0);
+        if (b == a.B - 1) seqs[a.B] = make_int2(0, row0 + s.n);
+      }
     }
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -176,7 +176,13 @@ __device__ __forceinline__ int find_seq(const int64_t* pre, int B, int64_t u) {
   return lo;
 }
 
-// Rows of a kv head and sequence above this run on the tile kernel.
+// Work is counted in 64 bits but hardly ever needs them.
+__device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
+  if (((a | b) >> 32) == 0) return (int64_t)((uint32_t)a / (uint32_t)b);
+  return a / b;
+}
+
+// More than 16 query rows of a kv head and sequence.
 template <int D, bool FP8>
 void launch_tiles(const Args& a, cudaStream_t stream);
 

@@ -216,12 +216,6 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* s
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, status, kStatusAttnTimeout, abort_flag));
 }
 
-// Work is counted in 64 bits but hardly ever needs them.
-__device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
-  if (((a | b) >> 32) == 0) return (int64_t)((uint32_t)a / (uint32_t)b);
-  return a / b;
-}
-
 // One CTA's share of one job: K / V tiles k0 .. k0 + nt of (sequence b, kv head h,
 // row tile).
 struct Segment {
@@ -502,7 +496,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tiles_kernel(const Args 
     tmem_alloc(&s_tmem, 512);
     tmem_relinquish();
   }
-  scan_work<kTok, kTileThreads>(a, kTileRows, pre, s_sum);
+  scan_work<kTok, kTileThreads>(a, kTileRows, a.Hkv, pre, s_sum);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -510,7 +504,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tiles_kernel(const Args 
   grid_dep_launch();
 
   const int64_t total = pre[a.B];
-  const int64_t piece = max((int64_t)1, (total + gridDim.x - 1) / gridDim.x);
+  const int64_t piece = max((int64_t)1, divide(total + gridDim.x - 1, gridDim.x));
   const int64_t u0 = (int64_t)blockIdx.x * piece;
   const int64_t u_end = min(total, u0 + piece);
   volatile int* abort_flag = &s_abort;
