@@ -11,14 +11,21 @@
 // different floats are so far apart that S is the number of values equal to
 // the maximum.
 //
-// Top k: each thread notes the chunk of its own largest value.  The k-th largest
-// of the threads' largest values is a bound below the row's k-th largest, and
-// only the at most k threads whose largest value reaches it can hold any of
-// the row's top k: their values alone are read a second time.  Order: larger
-// value first, then lower index (-0 = 0; a NaN comes before everything).
+// Top k: each thread notes the chunk of its own largest value.  Of the largest
+// values of 32 groups of threads the k-th is a bound below the row's k-th largest,
+// and only threads whose own largest value reaches it can hold any of the row's
+// top k: their values alone are read a second time, and the few that reach the bound
+// are ranked by counting, each against all.  (Sorting the threads' maxima instead, for
+// a tighter bound, cost more than the few values it spared.)  Order: larger value
+// first, then lower index (-0 = 0; a NaN comes before everything).
 //
 // A row is cut in slices, one for each CTA, when there are few rows; the last
 // CTA of a row joins them.
+//
+// Bound: memory for many rows (2047 rows of 128256 bf16 logits, 525 MB: 97 us without
+// alternatives, 5.4 TB/s; 110 us with one), where the exponentials take about 60 us and
+// 16-bit logits' maxima are taken two at a time.  Latency for few: one row 9 us with
+// alternatives, 64 rows 16 us, for two trips to memory, two joins of a CTA and a launch.
 #include <ATen/core/Tensor.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -113,6 +120,47 @@ __device__ __forceinline__ Key block_merge(Key v, Key* lists) {
   return lists[lane];
 }
 
+// The k-th largest of 32 groups' largest keys, groups by lane (the lowest indices of
+// equal values, in the first warp's chunks, are in groups of their own): at least k
+// keys reach it.  Zero if there are fewer than k groups with a key.
+__device__ __forceinline__ Key block_bound(Key key, int k, Key* lists) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  lists[threadIdx.x] = key;
+  __syncthreads();
+  if (warp == 0) {
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) {
+      const Key o = lists[w * 32 + lane];
+      key = o > key ? o : key;
+    }
+    __syncwarp();
+    lists[lane] = key;
+    __syncwarp();
+    int before = 0;
+#pragma unroll 8
+    for (int i = 0; i < 32; ++i) before += lists[i] > key || (lists[i] == key && i < lane);
+    __syncwarp();
+    if (before == k - 1) lists[0] = key;
+  }
+  __syncthreads();
+  return lists[0];
+}
+
+// Candidates by their place: out[0 .. k) = the k largest keys, descending (all
+// different; zeros after the last).
+__device__ __forceinline__ void block_rank(const Key* cand, int count, int k, Key* out) {
+  if (threadIdx.x < 32) out[threadIdx.x] = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < count; i += kThreads) {
+    const Key key = cand[i];
+    int before = 0;
+#pragma unroll 4
+    for (int j = 0; j < count; ++j) before += cand[j] > key;
+    if (before < k) out[before] = key;
+  }
+  __syncthreads();
+}
+
 // Running sums in the frame r; m is the largest value so far.
 struct Stat {
   float m, r, s, w;
@@ -156,11 +204,43 @@ __device__ __forceinline__ float value(const T* p) {
   else return __bfloat162float(*p);
 }
 
+__device__ __forceinline__ uint32_t max_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t max_nan_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
 // 16 bytes of logits as floats.
 template <typename T>
 struct Chunk {
   static constexpr int N = 16 / sizeof(T);
   float v[N];
+  // The largest of them, a NaN if there is one; with the values no lower than -1e30
+  // from here on if that comes cheap (`bounded`).
+  static constexpr bool bounded = std::is_same<T, __nv_bfloat16>::value;
+  __device__ __forceinline__ float set_top(uint4 u) {
+    if constexpr (bounded) {
+      const uint32_t t = max_nan_bf16x2(max_nan_bf16x2(u.x, u.y), max_nan_bf16x2(u.z, u.w));
+      constexpr uint32_t kLow = 0xf14af14au;  // -1e30, twice
+      u.x = max_bf16x2(u.x, kLow);
+      u.y = max_bf16x2(u.y, kLow);
+      u.z = max_bf16x2(u.z, kLow);
+      u.w = max_bf16x2(u.w, kLow);
+      set(u);
+      return max_nan(__uint_as_float(t << 16), __uint_as_float(t & 0xffff0000u));
+    } else {
+      set(u);
+      float top = v[0];
+#pragma unroll
+      for (int i = 1; i < N; ++i) top = max_nan(top, v[i]);
+      return top;
+    }
+  }
   __device__ __forceinline__ void set(const uint4& u) {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
@@ -179,14 +259,19 @@ struct Chunk {
   }
 };
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const Args a) {
+// CTAS of an SM: 2 leave a thread 64 registers, its loads of four chunks and the sums
+// of the last ones side by side; 3 are better where an SM works through many rows, and
+// the end of one hides behind the others (2047 rows of 128256: 110 us against 122;
+// 64 rows of 151936: 17.4 against 15.9).
+template <typename T, int CTAS>
+__global__ void __launch_bounds__(kThreads, CTAS) token_logprobs_kernel(const Args a) {
   constexpr int N = Chunk<T>::N;
   constexpr int U = 4;  // chunks in flight for each thread
   __shared__ Key lists[kThreads];
   __shared__ Key cand[kCand];
   __shared__ Stat stats[kWarps];
-  __shared__ int s_count, s_last;
+  __shared__ uint16_t owners[kThreads];
+  __shared__ int s_count, s_owners, s_last;
   grid_dep_launch();
   grid_dep_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -199,7 +284,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const Args a) 
   const int chunks = (hi - v0) / N;
   const int v1 = v0 + chunks * N;
   const uint4* xv = reinterpret_cast<const uint4*>(x + v0);
-  if (tid == 0) s_count = 0;
+  if (tid == 0) s_count = s_owners = 0;
 
   Stat st = {-INFINITY, kLowest, 0.f, 0.f};
   int best = tid;  // chunk of the largest value among the chunks
@@ -213,18 +298,16 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const Args a) 
     st.s *= f;
     st.r = r;
   };
-  auto add = [&](float v) {
-    const float d = fmaxf(fmaf(v, kLog2e, -st.r), -200.f);  // -inf: a weight of 0, not a NaN
+  auto add = [&](float v, bool bounded) {
+    float d = fmaf(v, kLog2e, -st.r);
+    if (!bounded) d = fmaxf(d, -200.f);  // -inf: a weight of 0, not a NaN
     const float e = ex2(d);
     st.s += e;
     st.w = fmaf(e, d, st.w);
   };
   auto take = [&](const uint4& raw, int c) {
     Chunk<T> u;
-    u.set(raw);
-    float top = u.v[0];
-#pragma unroll
-    for (int i = 1; i < N; ++i) top = max_nan(top, u.v[i]);
+    const float top = u.set_top(raw);
     nan |= top != top;
     if (top > best_v) {
       best_v = top;
@@ -232,7 +315,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const Args a) 
     }
     if (top * kLog2e > st.r + 8.f && top < kHuge) raise(top);
 #pragma unroll
-    for (int i = 0; i < N; ++i) add(u.v[i]);
+    for (int i = 0; i < N; ++i) add(u.v[i], Chunk<T>::bounded);
   };
   // Edges: fewer than 2 N elements, one for each of the first threads.
   const int n0 = v0 - lo;
@@ -242,7 +325,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const Args a) 
     edge_v = value(x + edge);
     nan |= edge_v != edge_v;
     if (edge_v > kLowest && edge_v < kHuge) raise(edge_v);
-    add(edge_v);
+    add(edge_v, false);
   }
   int c = tid;
   for (; c + (U - 1) * kThreads < chunks; c += U * kThreads) {
@@ -285,8 +368,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const Args a) 
   if (lane == 0) stats[warp] = st;
   Key top = 0;
   if (a.top_k > 0) {
-    const Key largest = block_merge(warp_sort(key), lists);
-    const Key bound = __shfl_sync(0xffffffffu, largest, a.top_k - 1);
+    const Key bound = block_bound(key, a.top_k, lists);
     auto offer = [&](Key k2) {
       if (k2 >= bound && k2 > 0) {
         const int at = atomicAdd(&s_count, 1);
@@ -294,26 +376,18 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const Args a) 
       }
     };
     if (edge >= 0) offer(make_key(edge_v, edge));
-    // The chunks of thread number j of the list, by one warp.
-    for (int j = warp; j < a.top_k; j += kWarps) {
-      const Key kj = __shfl_sync(0xffffffffu, largest, j);
-      if (kj == 0) break;
-      const int i = (int)~(uint32_t)kj;
-      const int owner = i < v0 ? i - lo : (i >= v1 ? n0 + i - v1 : ((i - v0) / N) % kThreads);
-      for (int at = owner + lane * kThreads; at < chunks; at += 32 * kThreads)
-        chunk_keys(at, offer);
+    if (key >= bound && key > 0) owners[atomicAdd(&s_owners, 1)] = (uint16_t)tid;
+    __syncthreads();
+    const int each = (chunks + kThreads - 1) / kThreads, all = s_owners * each;
+    for (int i = tid; i < all; i += kThreads) {
+      const int at = owners[i / each] + i % each * kThreads;
+      if (at < chunks) chunk_keys(at, offer);
     }
     __syncthreads();
     const int count = s_count;
-    if (count <= 128) {
-      if (warp == 0) {
-        for (int i = 0; i < count; i += 32)
-          top = warp_merge(top, warp_sort(i + lane < count ? cand[i + lane] : 0));
-      }
-    } else if (count <= kCand) {
-      for (int i = warp * 32; i < count; i += kThreads)
-        top = warp_merge(top, warp_sort(i + lane < count ? cand[i + lane] : 0));
-      top = block_merge(top, lists);
+    if (count <= kCand) {
+      block_rank(cand, count, a.top_k, lists);
+      top = lists[lane];
     } else {
       // More values over the bound than the list holds (many of a row's
       // largest values in a few threads' chunks): one pass for each place.
@@ -354,12 +428,29 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const Args a) 
     __threadfence();
     const float* parts = a.part + (int64_t)row * a.slices * P;
     if (a.top_k > 0) {
-      top = 0;
-      for (int i = warp; i < a.slices; i += kWarps) {
-        const Key* p = reinterpret_cast<const Key*>(parts + i * P + 4);
-        top = warp_merge(top, lane < a.top_k ? __ldcg(p + lane) : 0);
+      // The same again, with the slices' lists for the threads' chunks.
+      auto list = [&](int i) { return reinterpret_cast<const Key*>(parts + (int64_t)i * P + 4); };
+      if (tid == 0) s_count = 0;
+      key = 0;
+      for (int i = tid; i < a.slices; i += kThreads) keep_largest(__ldcg(list(i)));
+      const Key bound = block_bound(key, a.top_k, lists);
+      for (int i = tid; i < a.slices * a.top_k; i += kThreads) {
+        const Key k2 = __ldcg(list(i / a.top_k) + i % a.top_k);
+        if (k2 >= bound && k2 > 0) {
+          const int at = atomicAdd(&s_count, 1);
+          if (at < kCand) cand[at] = k2;
+        }
       }
-      top = block_merge(top, lists);
+      __syncthreads();
+      if (s_count <= kCand) {
+        block_rank(cand, s_count, a.top_k, lists);
+        top = lists[lane];
+      } else {
+        top = 0;
+        for (int i = warp; i < a.slices; i += kWarps)
+          top = warp_merge(top, lane < a.top_k ? __ldcg(list(i) + lane) : 0);
+        top = block_merge(top, lists);
+      }
     }
     if (warp == 0) {
       st = {-INFINITY, kLowest, 0.f, 0.f};
@@ -414,13 +505,23 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const Args a) 
   }
 }
 
+template <typename T>
+void launch(const Args& a, int rows, cudaStream_t stream) {
+  const dim3 grid((unsigned)a.slices, (unsigned)rows), block(kThreads);
+  if (rows >= 8 * num_sms())
+    launch_kernel(token_logprobs_kernel<T, 3>, grid, block, 0, stream, a);
+  else
+    launch_kernel(token_logprobs_kernel<T, 2>, grid, block, 0, stream, a);
+}
+
 }  // namespace lp
 
 // {slices of a row, workspace floats, workspace counters} of token_logprobs.
 std::vector<int64_t> token_logprobs_plan(int64_t rows, int64_t vocab, int64_t elem_size) {
-  // About four CTAs for each SM, slices of one chunk a thread at least.
+  // Two CTAs for each SM, all at once (64 rows, top 20: 15.9 us; three or four for each
+  // SM, that do not all fit, 22 and 27), slices of one chunk a thread at least.
   const int64_t least = lp::kThreads * (16 / elem_size);
-  int64_t s = std::max<int64_t>(1, 4 * num_sms() / std::max<int64_t>(1, rows));
+  int64_t s = std::max<int64_t>(1, 2 * num_sms() / std::max<int64_t>(1, rows));
   s = std::min(s, std::max<int64_t>(1, vocab / least));
   return {s, s > 1 ? rows * s * (4 + 2 * lp::kMaxTop) : 0, s > 1 ? rows : 0};
 }
@@ -466,13 +567,10 @@ void token_logprobs(at::Tensor logits, at::Tensor tokens, int64_t top_k,
   a.top_lp = top_lp.data_ptr<float>();
   a.part = ws.data_ptr<float>();
   a.counters = counters.data_ptr<int>();
-  const dim3 grid((unsigned)plan[0], (unsigned)R);
   cudaStream_t stream = at::cuda::getCurrentCUDAStream();
-  const dim3 block(lp::kThreads);
-  if (type == at::kFloat) launch_kernel(lp::token_logprobs_kernel<float>, grid, block, 0, stream, a);
-  else if (type == at::kHalf)
-    launch_kernel(lp::token_logprobs_kernel<__half>, grid, block, 0, stream, a);
-  else launch_kernel(lp::token_logprobs_kernel<__nv_bfloat16>, grid, block, 0, stream, a);
+  if (type == at::kFloat) lp::launch<float>(a, (int)R, stream);
+  else if (type == at::kHalf) lp::launch<__half>(a, (int)R, stream);
+  else lp::launch<__nv_bfloat16>(a, (int)R, stream);
 }
 
 }  // namespace cb
