@@ -8,6 +8,7 @@ the same math (used by the CPU engine and as test oracles) live in
 """
 from __future__ import annotations
 
+import functools
 import math
 import os
 import threading
@@ -282,6 +283,11 @@ def decode_split_plan(batch: int, kv_heads: int, max_blocks: int, num_sms: int =
     return splits, bps
 
 
+@functools.lru_cache(maxsize=16)
+def _attn_tree_plan(head_dim: int) -> tuple:
+    return tuple(ext().attn_tree_plan(head_dim)[1:])
+
+
 def attn_tree(q, k_cache, v_cache, block_tables, seq_lens, row_start, out, layer: int,
               scale: float, masks=None, k_scale=None, v_scale=None, max_nodes: int = 64,
               workspace: Optional[GemmWorkspace] = None):
@@ -300,12 +306,11 @@ def attn_tree(q, k_cache, v_cache, block_tables, seq_lens, row_start, out, layer
     if _dbg.ENABLED and not torch.cuda.is_current_stream_capturing():
         _dbg.check_paged(block_tables, seq_lens, k_cache.shape[1])
         _dbg.check_range("rows", row_start[1:] - row_start[:-1], 0, max_nodes + 1)
-    e = ext()
     ws = workspace or default_workspace(q.device)
-    plan = e.attn_tree_plan(k_cache.shape[4])
-    ws.ensure(plan[1], plan[2])
-    e.attn_tree(q, k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, row_start, masks,
-                out, layer, scale, max_nodes, ws.ws, ws.counters, status_buffer(q.device))
+    ws.ensure(*_attn_tree_plan(k_cache.shape[4]))
+    ext().attn_tree(q, k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, row_start,
+                    masks, out, layer, scale, max_nodes, ws.ws, ws.counters,
+                    status_buffer(q.device))
     LAUNCHES.add(1)
     return out
 
@@ -391,6 +396,11 @@ def kv_read_fp8(k_cache, v_cache, k_scale, v_scale, blocks, layer: int, k_out=No
     return k_out, v_out
 
 
+@functools.lru_cache(maxsize=256)
+def _logprobs_plan(rows: int, vocab: int, elem_size: int) -> tuple:
+    return tuple(ext().token_logprobs_plan(rows, vocab, elem_size)[1:])
+
+
 def token_logprobs(logits, tokens, top_k: int = 0, workspace: Optional[GemmWorkspace] = None):
     """Log-probabilities under softmax(logits): for every row of ``logits``
     ([R, V] bf16, fp16 or fp32, any row stride) the log-probability of its
@@ -403,18 +413,11 @@ def token_logprobs(logits, tokens, top_k: int = 0, workspace: Optional[GemmWorks
     NaN or +inf in the row gives NaN (a NaN ranks before every number), and so
     does a token outside the vocabulary."""
     R, V = logits.shape
-    e = ext()
-    dev = logits.device
-    plan = e.token_logprobs_plan(R, V, logits.element_size())
-    ws = workspace or default_workspace(dev)
-    ws.ensure(plan[1], plan[2])
-    lp = torch.empty(R, dtype=torch.float32, device=dev)
-    ent = torch.empty(R, dtype=torch.float32, device=dev)
-    ids = torch.empty(R, top_k, dtype=torch.int32, device=dev)
-    top = torch.empty(R, top_k, dtype=torch.float32, device=dev)
-    e.token_logprobs(logits, tokens, top_k, lp, ent, ids, top, ws.ws, ws.counters)
+    ws = workspace or default_workspace(logits.device)
+    ws.ensure(*_logprobs_plan(R, V, logits.element_size()))
+    out = ext().token_logprobs(logits, tokens, top_k, ws.ws, ws.counters)
     LAUNCHES.add(1)
-    return lp, ent, ids, top
+    return out
 
 
 def argmax(logits, out_idx, out_val=None, idx_offset: int = 0):

@@ -133,9 +133,9 @@ void attn_tree(torch::Tensor q, torch::Tensor k_cache, torch::Tensor v_cache,
                torch::Tensor status);
 // logprobs.cu
 std::vector<int64_t> token_logprobs_plan(int64_t rows, int64_t vocab, int64_t elem_size);
-void token_logprobs(torch::Tensor logits, torch::Tensor tokens, int64_t top_k,
-                    torch::Tensor logprob, torch::Tensor entropy, torch::Tensor top_ids,
-                    torch::Tensor top_lp, torch::Tensor ws, torch::Tensor counters);
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor> token_logprobs(
+    torch::Tensor logits, torch::Tensor tokens, int64_t top_k, torch::Tensor ws,
+    torch::Tensor counters);
 // elementwise.cu
 void embedding(torch::Tensor ids, torch::Tensor table, torch::Tensor out, int64_t vocab_lo);
 void rmsnorm(torch::Tensor x, c10::optional<torch::Tensor> residual, torch::Tensor w,

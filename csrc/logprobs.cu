@@ -27,6 +27,7 @@
 // 16-bit logits' maxima are taken two at a time.  Latency for few: one row 9 us with
 // alternatives, 64 rows 16 us, for two trips to memory, two joins of a CTA and a launch.
 #include <ATen/core/Tensor.h>
+#include <ATen/ops/empty.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
@@ -526,9 +527,10 @@ std::vector<int64_t> token_logprobs_plan(int64_t rows, int64_t vocab, int64_t el
   return {s, s > 1 ? rows * s * (4 + 2 * lp::kMaxTop) : 0, s > 1 ? rows : 0};
 }
 
-void token_logprobs(at::Tensor logits, at::Tensor tokens, int64_t top_k,
-                    at::Tensor logprob, at::Tensor entropy, at::Tensor top_ids,
-                    at::Tensor top_lp, at::Tensor ws, at::Tensor counters) {
+// Log-probability [R], entropy [R], ids of the top alternatives [R, k] and theirs.
+// (The results are allocated here: from Python that took longer than one row does.)
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> token_logprobs(
+    at::Tensor logits, at::Tensor tokens, int64_t top_k, at::Tensor ws, at::Tensor counters) {
   TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && logits.stride(1) == 1 && logits.size(1) > 0,
               "logits must be [rows, vocab] with inner stride 1");
   const auto type = logits.scalar_type();
@@ -541,18 +543,19 @@ void token_logprobs(at::Tensor logits, at::Tensor tokens, int64_t top_k,
   TORCH_CHECK(tokens.scalar_type() == at::kInt && tokens.is_contiguous() && tokens.numel() == R &&
                   tokens.device() == logits.device(),
               "tokens must be int32, one per row");
-  TORCH_CHECK(logprob.scalar_type() == at::kFloat && entropy.scalar_type() == at::kFloat &&
-                  top_ids.scalar_type() == at::kInt && top_lp.scalar_type() == at::kFloat &&
-                  logprob.numel() >= R && entropy.numel() >= R && top_ids.numel() >= R * top_k &&
-                  top_lp.numel() >= R * top_k && logprob.is_contiguous() &&
-                  entropy.is_contiguous() && top_ids.is_contiguous() && top_lp.is_contiguous(),
-              "outputs must be contiguous fp32 [R], [R], int32 [R, k], fp32 [R, k]");
-  if (R == 0) return;
   TORCH_CHECK(R <= 65535, "at most 65535 rows in one call");
   const c10::cuda::CUDAGuard guard(logits.device());
+  const auto f32 = logits.options().dtype(at::kFloat);
+  at::Tensor logprob = at::empty({R}, f32), entropy = at::empty({R}, f32);
+  at::Tensor top_ids = at::empty({R, top_k}, f32.dtype(at::kInt));
+  at::Tensor top_lp = at::empty({R, top_k}, f32);
+  if (R == 0) return {logprob, entropy, top_ids, top_lp};
   const int64_t es = (int64_t)logits.element_size();
   const std::vector<int64_t> plan = token_logprobs_plan(R, V, es);
-  TORCH_CHECK(ws.numel() >= plan[1] && counters.numel() >= plan[2], "workspace too small");
+  TORCH_CHECK(ws.scalar_type() == at::kFloat && counters.scalar_type() == at::kInt &&
+                  ws.device() == logits.device() && counters.device() == logits.device() &&
+                  ws.numel() >= plan[1] && counters.numel() >= plan[2],
+              "workspace too small");
   lp::Args a;
   a.x = logits.data_ptr();
   a.ld = logits.stride(0);
@@ -571,6 +574,7 @@ void token_logprobs(at::Tensor logits, at::Tensor tokens, int64_t top_k,
   if (type == at::kFloat) lp::launch<float>(a, (int)R, stream);
   else if (type == at::kHalf) lp::launch<__half>(a, (int)R, stream);
   else lp::launch<__nv_bfloat16>(a, (int)R, stream);
+  return {logprob, entropy, top_ids, top_lp};
 }
 
 }  // namespace cb
