@@ -69,14 +69,6 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], u
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Four codes as fp16: those of the word's lower half, those of its upper half.
-__device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  asm("{\n.reg .b16 a, b;\nmov.b32 {a, b}, %2;\ncvt.rn.f16x2.e4m3x2 %0, a;\n"
-      "cvt.rn.f16x2.e4m3x2 %1, b;\n}"
-      : "=r"(lo), "=r"(hi)
-      : "r"(w));
-}
-
 constexpr float kLag = 2.f;   // scores may pass the maximum in use by a factor 2^kLag
 constexpr float kUp = 13.f;   // fp16 weights are held as 2^kUp w: at most 2^(kUp + kLag)
 constexpr float kSum = 8.f;   // and summed as 2^kSum w / vs
@@ -863,6 +855,7 @@ void attn_tree(at::Tensor q, at::Tensor k_cache, at::Tensor v_cache,
   a.B = (int)B;
   a.Hkv = Hkv;
   a.G = (int)(q.size(1) / D / Hkv);
+  a.per_g = a.G == 1 ? 0u : (uint32_t)(((1ull << 32) + a.G - 1) / a.G);
   a.scale_log2 = (float)scale * tree::kLog2e;
   cudaStream_t stream = at::cuda::getCurrentCUDAStream();
   const int64_t rows = max_nodes * a.G;

@@ -37,19 +37,19 @@ struct Args {
   int* status;
   int64_t layer_blocks;
   int B, Hkv, G;
+  uint32_t per_g;  // 2^32 / G, rounded up; 0 for G = 1
   int out_vec;  // output rows are 16-byte aligned
   float scale_log2;
 };
 
-// 4 e4m3 codes as fp16 times 2^-8, exact: the exponent and mantissa bits move
-// into place, the biases differ by 8 and e4m3's subnormals become fp16's.  even
-// holds codes 0 and 2 of the word, odd 1 and 3.  Seven integer instructions for
-// four codes; the conversion instruction runs on the unit that computes the
-// exponentials.  The code of a NaN does not come out as one; the writer never
-// stores it.
-__device__ __forceinline__ void e4m3_to_f16(uint32_t w, uint32_t& even, uint32_t& odd) {
-  even = ((w << 8) & 0x80008000u) | ((w << 7) & 0x3f803f80u);
-  odd = (w & 0x80008000u) | ((w >> 1) & 0x3f803f80u);
+// Four codes as fp16, exact: those of the word's lower half, those of its upper half.
+// (The conversion runs at the rate of an integer instruction; moving the bits into place
+// takes three and a half for every pair.)
+__device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  asm("{\n.reg .b16 a, b;\nmov.b32 {a, b}, %2;\ncvt.rn.f16x2.e4m3x2 %0, a;\n"
+      "cvt.rn.f16x2.e4m3x2 %1, b;\n}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(w));
 }
 
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
@@ -108,6 +108,11 @@ __device__ __forceinline__ uint4 ldg_stream16(const void* p) {
                : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
                : "l"(p));
   return v;
+}
+
+// Node of a query row, node * G + head of the group, below 2^32 / G.
+__device__ __forceinline__ int node_of(const Args& a, int r) {
+  return a.G == 1 ? r : (int)__umulhi((uint32_t)r, a.per_g);
 }
 
 // n rows, len keys in nb units of UNIT tokens (one at least), read by `tiles`

@@ -176,6 +176,9 @@ __device__ __forceinline__ uint32_t lds32(uint32_t addr) {
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
   return v;
 }
+__device__ __forceinline__ void sts64(uint32_t addr, uint32_t a, uint32_t b) {
+  asm volatile("st.shared.v2.b32 [%0], {%1,%2};" ::"r"(addr), "r"(a), "r"(b) : "memory");
+}
 __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
   uint32_t r;
   asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
@@ -213,7 +216,8 @@ struct RowSight {
 // A wait of a whole warp: the warp stays together, and gives up together.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* status,
                                           volatile int* abort_flag) {
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity, status, kStatusAttnTimeout, abort_flag));
+  return __all_sync(
+      0xffffffffu, mbar_wait_sleep(bar, parity, status, kStatusAttnTimeout, abort_flag));
 }
 
 // One CTA's share of one job: K / V tiles k0 .. k0 + nt of (sequence b, kv head h,
@@ -361,7 +365,7 @@ __device__ __forceinline__ void load_tiles(const Args& a, const int64_t* pre, in
         // far from overflow then, even for heads whose values are all zero.
         top = __reduce_max_sync(0xffffffffu, top);
         const int x = top == 0u ? 127 : max(43, (int)(top >> 23));
-        const float factor = __int_as_float((253 - x) << 23) * 16384.f;  // 2^14 / reference
+        const float factor = __int_as_float((253 - x) << 23) * 64.f;  // 2^6 / reference
         uint32_t pair[4];  // each token's scale over the reference as two fp16 numbers
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -409,12 +413,13 @@ __device__ __forceinline__ void load_tiles(const Args& a, const int64_t* pre, in
           else if (more) vb[i] = load_row(k_base + v_minus_k, i, next_pages);
           const uint32_t c0 = v_dst + tok * 128 + ((v_chunk ^ (tok & 7)) << 4);
           if constexpr (FP8) {
-            // Codes unpack times 2^-8, scales are at most 2^14: 448 x 2^6 at most.
+            // Scales are at most 2^6: values of 448 x 2^6 at most.
             const uint32_t pair = lds32(sm.pairs + tok * 4);
             const uint32_t hi = __byte_perm(pair, 0u, 0x1010), lo = __byte_perm(pair, 0u, 0x3232);
+            if (tail && pair == 0u) w[0] = w[1] = w[2] = w[3] = 0u;  // codes may be NaN's there
             uint32_t f[8];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) e4m3_to_f16(w[j], f[2 * j], f[2 * j + 1]);
+            for (int j = 0; j < 4; ++j) codes_to_f16(w[j], f[2 * j], f[2 * j + 1]);
 #pragma unroll
             for (int j = 0; j < 8; ++j) f[j] = hfma2(f[j], hi, hmul2(f[j], lo));
             sts128(c0, f[0], f[1], f[2], f[3]);
@@ -621,53 +626,77 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tiles_kernel(const Args 
     for (int64_t u = u0; u < u_end;) {
       const Segment g = segment_at(a, pre, u, u_end, piece, *abort_flag != 0);
       u += g.units;
-      // This thread's row, its query into shared memory.
+      // This thread's row.
       const int row = g.mt == 2 ? tid : tid & 127;
       const bool live_row = row < g.rows;
       const bool live_warp = (g.mt == 2 ? warp : warp & 3) * 32 < g.rows;
       const int rr = g.row0 + (live_row ? row : 0);
-      const int node = rr / a.G;
+      const int node = node_of(a, rr);
       const int64_t q_row = g.q_row0 + node;
-      const int head = g.h * a.G + rr % a.G;
+      const int head = g.h * a.G + rr - node * a.G;
       float row_scale = a.scale_log2;
+      // The warp's 32 query rows into shared memory, D / 8 lanes a row.  (Each thread
+      // its own row instead: 32 lines an instruction, 5 us before the first product.)
       {
-        uint4 y[D / 8];
-        const __nv_bfloat16* qp = a.q + q_row * a.q_stride + (int64_t)head * D;
-        uint32_t top = 0;
-#pragma unroll
-        for (int c = 0; c < D / 8; ++c)
-          y[c] = live_row ? *reinterpret_cast<const uint4*>(qp + 8 * c) : make_uint4(0u, 0u, 0u, 0u);
+        constexpr int LPR = D / 8, RPI = 32 / LPR;  // lanes of a row, rows of a load
+        const int lane = tid & 31, c = lane % LPR, sub = lane / LPR;
+        const int first = (g.mt == 2 ? warp : warp & 3) * 32;  // its row in the job
         const bool writes = g.mt == 2 || wg == 0;
-        const uint32_t dst =
-            smem_u32(smem + S::kQ) + (g.mt == 2 ? wg : 0) * S::kQTile + (tid & 127) * 128;
-        const int r = tid & 7;
-        if constexpr (FP8) {
+        const uint32_t dst = smem_u32(smem + S::kQ) + (g.mt == 2 ? wg : 0) * S::kQTile;
+        const __nv_bfloat16* q_base =
+            a.q + (int64_t)g.q_row0 * a.q_stride + (int64_t)g.h * a.G * D + 8 * c;
+        constexpr int kBatch = 8;  // loads in flight
+#pragma unroll 1
+        for (int i0 = 0; i0 < 32 / RPI; i0 += kBatch) {
+          uint4 y[kBatch];
 #pragma unroll
-          for (int c = 0; c < D / 8; ++c) {
-            const uint32_t w[4] = {y[c].x, y[c].y, y[c].z, y[c].w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              top = max(top, max(w[i] & 0x7fffu, (w[i] >> 16) & 0x7fffu));
+          for (int i = 0; i < kBatch; ++i) {
+            const int r = first + (i0 + i) * RPI + sub;
+            const int node = node_of(a, g.row0 + r);
+            y[i] = make_uint4(0u, 0u, 0u, 0u);
+            if (r < g.rows)
+              y[i] = *reinterpret_cast<const uint4*>(
+                  q_base + node * a.q_stride + (g.row0 + r - node * a.G) * D);
           }
-          const QScale qs = q_scale(top);
-          row_scale *= qs.down;
+          float up[kBatch];
+          if constexpr (FP8) {
+            uint32_t top[kBatch];
 #pragma unroll
-          for (int c = 0; c < D / 8; c += 2) {
-            uint32_t hi[4], lo[4];
-            split_e4m3(y[c].x, y[c].y, qs.up, hi[0], lo[0]);
-            split_e4m3(y[c].z, y[c].w, qs.up, hi[1], lo[1]);
-            split_e4m3(y[c + 1].x, y[c + 1].y, qs.up, hi[2], lo[2]);
-            split_e4m3(y[c + 1].z, y[c + 1].w, qs.up, hi[3], lo[3]);
-            if (writes) {
-              const uint32_t at = dst + (((c >> 1) ^ r) << 4);
-              sts128(at, hi[0], hi[1], hi[2], hi[3]);
-              sts128(at + kSlab, lo[0], lo[1], lo[2], lo[3]);
+            for (int i = 0; i < kBatch; ++i) {
+              const uint32_t both = __vmaxu2(__vmaxu2(y[i].x & 0x7fff7fffu, y[i].y & 0x7fff7fffu),
+                                             __vmaxu2(y[i].z & 0x7fff7fffu, y[i].w & 0x7fff7fffu));
+              top[i] = max(both & 0xffffu, both >> 16);
+            }
+#pragma unroll
+            for (int o = 1; o < LPR; o <<= 1)
+#pragma unroll
+              for (int i = 0; i < kBatch; ++i)
+                top[i] = max(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+              const QScale qs = q_scale(top[i]);
+              up[i] = qs.up;
+              // (for the thread that has this row)
+              const float down = __shfl_sync(0xffffffffu, qs.down, lane % RPI * LPR);
+              if (lane / RPI == i0 + i) row_scale *= down;
             }
           }
-        } else if (writes) {
+          if (!writes) continue;
 #pragma unroll
-          for (int c = 0; c < D / 8; ++c)
-            sts128(dst + (c >> 3) * kSlab + (((c & 7) ^ r) << 4), y[c].x, y[c].y, y[c].z, y[c].w);
+          for (int i = 0; i < kBatch; ++i) {
+            const int r = (first + (i0 + i) * RPI + sub) & 127;
+            if constexpr (FP8) {
+              uint32_t hi[2], lo[2];
+              split_e4m3(y[i].x, y[i].y, up[i], hi[0], lo[0]);
+              split_e4m3(y[i].z, y[i].w, up[i], hi[1], lo[1]);
+              const uint32_t at = dst + r * 128 + (((c >> 1) ^ (r & 7)) << 4) + (c & 1) * 8;
+              sts64(at, hi[0], hi[1]);
+              sts64(at + kSlab, lo[0], lo[1]);
+            } else {
+              sts128(dst + (c >> 3) * kSlab + r * 128 + (((c & 7) ^ (r & 7)) << 4), y[i].x, y[i].y,
+                     y[i].z, y[i].w);
+            }
+          }
         }
         fence_proxy_async_smem();
         tc_fence_before();
@@ -844,9 +873,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tiles_kernel(const Args 
         for (int i = 0; i < 16; ++i) y[i] = none ? 0.f : y[i] * inv;
 #pragma unroll
         for (int i = 0; i < 16; i += 4) {
-          // (8-bit values come with dims 0, 2, 1, 3 of every four)
-          w[i / 2] = FP8 ? pack_bf16(y[i], y[i + 2]) : pack_bf16(y[i], y[i + 1]);
-          w[i / 2 + 1] = FP8 ? pack_bf16(y[i + 1], y[i + 3]) : pack_bf16(y[i + 2], y[i + 3]);
+          w[i / 2] = pack_bf16(y[i], y[i + 1]);
+          w[i / 2 + 1] = pack_bf16(y[i + 2], y[i + 3]);
         }
         __nv_bfloat16* dst = a.out + q_row * a.out_stride + (int64_t)head * D + d;
         if (a.out_vec) {
