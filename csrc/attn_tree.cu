@@ -87,10 +87,6 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
   return r;
 }
 
-// Asynchronous copies global -> shared, each lane for itself.
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
 __device__ __forceinline__ float lds32(uint32_t p) {
   float v;
   asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(p) : "memory");
@@ -101,12 +97,6 @@ __device__ __forceinline__ uint2 lds64(uint32_t p) {
   asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(p) : "memory");
   return v;
 }
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copies_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
 // One warp's view of one 16-token block: K and V words and the scales.
 //
 // Tokens of lane (g, t4): K rows g and 8 + g (their scales too); V rows 2 t4, 2 t4 + 1
@@ -757,7 +747,10 @@ void launch_rows(const Args& a, cudaStream_t stream) {
   launch_kernel(attn_rows_kernel<D, FP8, NR>, dim3(per_head * a.Hkv), dim3(128), smem, stream, a);
 }
 
-// By the query rows of a kv head and sequence.
+// By the query rows of a kv head and sequence.  64 sequences of 2048 keys, 8 kv heads
+// of 128, 8-bit cache (bf16): 8 rows 59 us here and 78 with room for 16 (93 and 94); 16
+// rows 100 and 85 (169 and 101), 143 on the tile kernel (124); 20 rows 147 here, where
+// they read the keys twice, and 143 on the tile kernel (179 and 126).
 template <int D, bool FP8>
 void launch(const Args& a, int64_t max_rows, cudaStream_t stream) {
   if (max_rows <= 8)

@@ -3,9 +3,8 @@
 //
 // One CTA an SM:
 //   warps 0-3, 4-7  softmax, one thread a row;
-//   warps 8-15      K and V: global memory -> registers -> shared memory in the
-//                   128-byte swizzle, two stages of 128 tokens, 64 tokens for each
-//                   four warps;
+//   warps 8-15      K and V: global memory -> shared memory in the 128-byte swizzle,
+//                   two stages of 128 tokens, 64 tokens for each four warps;
 //   warps 16-19     one thread of each issues the products.
 // Tensor memory (512 columns): for each softmax group the scores of two steps of 64
 // tokens and the sums.  S = Q K^T reads both operands from shared memory; the weights
@@ -32,6 +31,12 @@
 // the tile are hidden) the tile is taken again in two passes and the sums are
 // rescaled.  Weights thus stay below 2^8: fp16 weights are held as 2^7 w, below
 // 2^15.
+//
+// Bound: the softmax threads' own time, 2100 cycles for a step of 64 tokens and 700
+// for its waits, while the products take about 800 and the loads less.  8 trees of 64
+// nodes x 4 heads over 8192 keys, 8 kv heads of 128, 8-bit cache: 160 us, 425 TFLOP/s
+// (134 MB).  With one row tile the loading warps, 3000 cycles for 128 tokens of the
+// 8-bit cache: 64 sequences of 2048 keys, 20 rows, 143 us (bf16 cache 126 us, 4.3 TB/s).
 #include "attn_tree.cuh"
 #include "common.cuh"
 #include "host_utils.h"
@@ -62,7 +67,8 @@ struct TileSmem {
   static constexpr int kK = 0;                       // [2]
   static constexpr int kV = kK + 2 * kKTile;         // [2]
   static constexpr int kQ = kV + 2 * kVTile;         // [2]
-  static constexpr int kScale = kQ + 2 * kQTile;     // K's: [kTileBufs][128] fp32
+  static constexpr int kRaw = kQ + 2 * kQTile;       // V's codes as they come: [2][128][D]
+  static constexpr int kScale = kRaw + (FP8 ? 2 * 128 * D : 0);  // K's: [kTileBufs][128] fp32
   static constexpr int kPairs = kScale + kTileBufs * kTok * 4;  // V's: [8 warps][128]
   static constexpr int kMl = kPairs + 8 * kTok * 4;  // [2][128][2]
   static constexpr int kBars = kMl + 2 * 128 * 2 * 4;
@@ -266,6 +272,7 @@ __device__ __forceinline__ Segment segment_at(const Args& a, const int64_t* pre,
 // What the loading groups share with the others.
 struct LoadSmem {
   uint32_t k, v;      // [2] operand tiles (shared addresses)
+  uint32_t raw;       // this lane's place in V's codes
   uint32_t pairs;     // this warp's [128] scales of V over the reference, as fp16 pairs
   float* k_scale;     // [kTileBufs][128]
   float* v_ref;       // [kTileBufs]: log2 of V's reference / 2^6
@@ -276,8 +283,10 @@ struct LoadSmem {
 };
 
 // Four warps bring 64 tokens of every K / V tile of the CTA's jobs into shared
-// memory.  As a row is stored, the same row of the next tile takes its registers,
-// so that half a tile's loads are always in flight for each group.
+// memory, by asynchronous copies: K, and V of the bf16 cache, to their places; V's codes
+// to a place of the lane's own, whence it unpacks them.  The next tile's copies are made
+// as soon as there is room.  (Loads into registers, a tile ahead, kept waiting for one
+// another: a warp has but a few counters for all its loads in flight.)
 template <int D, bool FP8>
 __device__ __forceinline__ void load_tiles(const Args& a, const int64_t* pre, int64_t u0,
                                            int64_t u_end, int64_t piece, const LoadSmem& sm,
@@ -286,9 +295,7 @@ __device__ __forceinline__ void load_tiles(const Args& a, const int64_t* pre, in
   constexpr int RB = FP8 ? D : 2 * D;      // bytes of a cache row
   constexpr int LPT = RB / 16;             // lanes that share a row, 16 bytes each
   constexpr int TPW = 32 / LPT;            // rows of one warp-wide load
-  constexpr int ROWS = 64 / (4 * TPW);     // loads of a lane for its part of a tile
-  constexpr int NI = ROWS < 4 ? ROWS : 4;  // of them in flight, of K and of V
-  constexpr int PARTS = ROWS / NI;
+  constexpr int ROWS = 64 / (4 * TPW);     // copies of a lane for its part of a tile, of K and of V
   const int ct = threadIdx.x & 127, cw = ct >> 5, lane = ct & 31;
   // Lanes in fours along a row, then over two rows: the eight lanes of a store
   // phase then write different banks, also when each writes every other chunk.
@@ -310,16 +317,37 @@ __device__ __forceinline__ void load_tiles(const Args& a, const int64_t* pre, in
     const int blocks = (g.len + 15) >> 4;
     const int64_t first_row = (a.layer_blocks * a.Hkv + g.h) * 16;
     const uint8_t* k_base = a.k + first_row * RB + piece16 * 16;
-    const int64_t v_minus_k = a.v - a.k;
+    const uint8_t* v_base = a.v + first_row * RB + piece16 * 16;
     // Blocks past the end read the last one (hidden, and zeroed where it would
     // matter).
     auto fetch_pages = [&](int kt) {
       return __ldg(g.table + min((g.k0 + kt) * 8 + (lane & 7), blocks - 1));
     };
-    auto load_row = [&](const uint8_t* base, int i, int pages) {
-      const int tok = token_of(i);
-      const int page = __shfl_sync(0xffffffffu, pages, tok >> 4);
-      return ldg_stream16(base + page * block_bytes + (tok & 15) * RB);
+    auto row_at = [&](int tok, int pages) {
+      const int64_t page = __shfl_sync(0xffffffffu, pages, tok >> 4);
+      return page * block_bytes + (tok & 15) * RB;
+    };
+    // Room for a tile (of all the CTA's tiles), its copies.
+    auto room = [&](uint64_t* free, int tile) {
+      return tile < 2 ||
+             warp_wait(free + (tile & 1), ((tile >> 1) + 1) & 1, a.status, sm.abort_flag);
+    };
+    auto copy_k = [&](int tile, int pages) {
+      const uint32_t dst = k_tiles + (tile & 1) * S::kKTile;
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i) {
+        const int tok = token_of(i);
+        copy16(dst + tok * 128 + ((k_chunk ^ (tok & 7)) << 4), k_base + row_at(tok, pages));
+      }
+    };
+    auto copy_v = [&](int tile, int pages) {
+      const uint32_t dst = FP8 ? sm.raw + (tile & 1) * 128 * D : v_tiles + (tile & 1) * S::kVTile;
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i) {
+        const int tok = token_of(i);
+        copy16(FP8 ? dst + i * 512 : dst + tok * 128 + ((v_chunk ^ (tok & 7)) << 4),
+               v_base + row_at(tok, pages));
+      }
     };
     // Scales of tokens 4 lane .. 4 lane + 3 of a tile.
     auto load_scales = [&](const float* from, int pages) {
@@ -327,22 +355,21 @@ __device__ __forceinline__ void load_tiles(const Args& a, const int64_t* pre, in
       return __ldg(reinterpret_cast<const float4*>(from + first_row + page * a.Hkv * 16) +
                    (lane & 3));
     };
-    uint4 kb[NI], vb[NI];
     float4 ks = make_float4(0.f, 0.f, 0.f, 0.f), vs = ks;
     // Page numbers run ahead of the rows they lead to.
     int pages = fetch_pages(0), next_pages = fetch_pages(1);
-#pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      kb[i] = load_row(k_base, i, pages);
-      vb[i] = load_row(k_base + v_minus_k, i, pages);
-    }
+    if (!room(sm.k_free, kc)) continue;
+    copy_k(kc, pages);
+    copies_commit();
+    if (!FP8 && !room(sm.v_free, kc)) continue;
+    copy_v(kc, pages);
+    copies_commit();
     if constexpr (FP8) {
       ks = load_scales(a.ks, pages);
       vs = load_scales(a.vs, pages);
     }
     for (int kt = 0; kt < g.nt; ++kt, ++kc) {
       const int st = kc & 1;
-      const uint32_t parity = ((kc >> 1) + 1) & 1;
       const bool more = kt + 1 < g.nt;
       const int later_pages = fetch_pages(kt + 2);
       const int pos0 = (g.k0 + kt) * kTok;
@@ -387,31 +414,24 @@ __device__ __forceinline__ void load_tiles(const Args& a, const int64_t* pre, in
           vs = load_scales(a.vs, next_pages);
         }
       }
-      if (kc >= 2 && !warp_wait(sm.k_free + st, parity, a.status, sm.abort_flag)) break;
-      const uint32_t k_dst = k_tiles + st * S::kKTile;
-#pragma unroll
-      for (int part = 0; part < PARTS; ++part)
-#pragma unroll
-        for (int i = 0; i < NI; ++i) {
-          const int tok = token_of(part * NI + i);
-          const uint4 w = kb[i];
-          if (part + 1 < PARTS) kb[i] = load_row(k_base, (part + 1) * NI + i, pages);
-          else if (more) kb[i] = load_row(k_base, i, next_pages);
-          sts128(k_dst + tok * 128 + ((k_chunk ^ (tok & 7)) << 4), w.x, w.y, w.z, w.w);
-        }
+      copies_wait<1>();
       fence_proxy_async_smem();
       mbar_arrive(sm.k_full + st);
-      if (kc >= 2 && !warp_wait(sm.v_free + st, parity, a.status, sm.abort_flag)) break;
+      if (more) {
+        if (!room(sm.k_free, kc + 1)) break;
+        copy_k(kc + 1, next_pages);
+      }
+      copies_commit();
+      copies_wait<1>();
       const uint32_t v_dst = v_tiles + st * S::kVTile;
+      if (FP8 && !room(sm.v_free, kc)) break;
+      if (FP8 || tail) {
 #pragma unroll
-      for (int part = 0; part < PARTS; ++part)
-#pragma unroll
-        for (int i = 0; i < NI; ++i) {
-          const int tok = token_of(part * NI + i);
-          uint32_t w[4] = {vb[i].x, vb[i].y, vb[i].z, vb[i].w};
-          if (part + 1 < PARTS) vb[i] = load_row(k_base + v_minus_k, (part + 1) * NI + i, pages);
-          else if (more) vb[i] = load_row(k_base + v_minus_k, i, next_pages);
+        for (int i = 0; i < ROWS; ++i) {
+          const int tok = token_of(i);
           const uint32_t c0 = v_dst + tok * 128 + ((v_chunk ^ (tok & 7)) << 4);
+          const uint4 u = lds128(FP8 ? sm.raw + st * 128 * D + i * 512 : c0);
+          uint32_t w[4] = {u.x, u.y, u.z, u.w};
           if constexpr (FP8) {
             // Scales are at most 2^6: values of 448 x 2^6 at most.
             const uint32_t pair = lds32(sm.pairs + tok * 4);
@@ -425,28 +445,33 @@ __device__ __forceinline__ void load_tiles(const Args& a, const int64_t* pre, in
             sts128(c0, f[0], f[1], f[2], f[3]);
             sts128(c0 ^ 16u, f[4], f[5], f[6], f[7]);
           } else {
-            if (tail) {
-              // Value rows that a product must not meet: past the end anything may
-              // lie there, and a node may hold an infinity or a NaN that its
-              // siblings do not see (added to the rows that do see it at the end).
-              bool bad = false;
+            // Value rows that a product must not meet: past the end anything may
+            // lie there, and a node may hold an infinity or a NaN that its
+            // siblings do not see (added to the rows that do see it at the end).
+            bool bad = false;
 #pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                if (pos0 + tok >= g.len) w[j] = 0u;
-                if ((w[j] & 0x7f80u) == 0x7f80u) { w[j] &= 0xffff0000u; bad = true; }
-                if ((w[j] & 0x7f800000u) == 0x7f800000u) { w[j] &= 0xffffu; bad = true; }
-              }
-              if (bad) *sm.nonfinite = 1;
+            for (int j = 0; j < 4; ++j) {
+              if (pos0 + tok >= g.len) w[j] = 0u;
+              if ((w[j] & 0x7f80u) == 0x7f80u) { w[j] &= 0xffff0000u; bad = true; }
+              if ((w[j] & 0x7f800000u) == 0x7f800000u) { w[j] &= 0xffffu; bad = true; }
             }
+            if (bad) *sm.nonfinite = 1;
             sts128(c0, w[0], w[1], w[2], w[3]);
           }
         }
+      }
       fence_proxy_async_smem();
       mbar_arrive(sm.v_full + st);
+      if (more) {
+        if (!FP8 && !room(sm.v_free, kc + 1)) break;
+        copy_v(kc + 1, next_pages);
+      }
+      copies_commit();
       pages = next_pages;
       next_pages = later_pages;
     }
   }
+  copies_wait<0>();
 }
 
 template <int D, bool FP8>
@@ -605,6 +630,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tiles_kernel(const Args 
     LoadSmem sm;
     sm.k = smem_u32(smem + S::kK);
     sm.v = smem_u32(smem + S::kV);
+    sm.raw = smem_u32(smem + S::kRaw) + (warp - 8) * 16 * D + (tid & 31) * 16;
     sm.pairs = smem_u32(smem + S::kPairs) + (warp - 8) * kTok * 4;
     sm.k_scale = k_scale;
     sm.v_ref = s_vref;

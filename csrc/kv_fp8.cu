@@ -264,7 +264,9 @@ static void check_fp8_cache(const at::Tensor& k, const at::Tensor& v,
 }
 
 // Few tokens: one head a thread, so that the heads' loads and the row maxima of
-// one token run side by side; from four CTAs an SM on, three heads a thread.
+// one token run side by side; from four CTAs an SM on, three heads a thread, with more
+// loads in flight (32 + 2 x 8 heads of 128; 64 tokens: 1.9 us against 2.3, 592: 3.4
+// against 4.1; 1024: 4.8 against 4.2, 8192: 35 against 33).
 template <int D>
 static void launch_write(const WriteArgs& a, cudaStream_t stream) {
   constexpr int groups = 128 / (D / 16);
