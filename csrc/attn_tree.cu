@@ -823,8 +823,9 @@ void attn_tree(at::Tensor q, at::Tensor k_cache, at::Tensor v_cache,
   const c10::cuda::CUDAGuard guard(q.device());
   const std::vector<int64_t> plan = attn_tree_plan(D);
   TORCH_CHECK(ws.scalar_type() == at::kFloat && ws.numel() >= plan[1] &&
-                  counters.scalar_type() == at::kInt && counters.numel() >= plan[2],
-              "workspace too small");
+                  counters.scalar_type() == at::kInt && counters.numel() >= plan[2] &&
+                  reinterpret_cast<uintptr_t>(ws.data_ptr()) % 16 == 0,
+              "workspace too small, or not 16-byte aligned");
   tree::Args a;
   a.q = reinterpret_cast<const __nv_bfloat16*>(q.data_ptr());
   a.q_stride = q.stride(0);

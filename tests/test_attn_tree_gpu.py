@@ -373,3 +373,30 @@ def test_refusals():
                                         q=torch.zeros(2, 512, dtype=torch.bfloat16, device=DEV),
                                         out=torch.zeros(2, 512, dtype=torch.bfloat16, device=DEV),
                                         layer=0)})
+
+
+@pytest.mark.parametrize("cache", ["fp8", "bf16"])
+@pytest.mark.parametrize("hq,hkv,d,most", [(6, 3, 128, 1), (6, 3, 64, 4), (10, 5, 128, 6)])
+def test_pieces_across_sequences(cache, hq, hkv, d, most):
+    """Contexts from nothing to some hundred keys: a CTA's piece holds ends, middles and
+    whole sequences, with fewer blocks than its warps or many more."""
+    g = torch.Generator().manual_seed(31)
+    lens = torch.randint(0, 40, (260,), generator=g).tolist()
+    lens[::7] = torch.randint(100, 1200, (len(lens[::7]),), generator=g).tolist()
+    nodes = [min(n, 1 + i % most) if i % 11 else 0 for i, n in enumerate(lens)]
+    p = Problem(cache, hq, hkv, d, lens, nodes, tree=most > 1, seed=d + most)
+    p.check(p.run())
+
+
+def test_refuses_a_misaligned_workspace():
+    p = Problem("bf16", 4, 2, 64, [20], [1], seed=4)
+    ws = ops.GemmWorkspace(DEV)
+    whole = ws.ws
+    ws.ws = whole[1:]
+    kw = dict(layer=1, scale=0.125, max_nodes=1, workspace=ws)
+    args = (p.q.to(DEV), p.kc, p.vc, p.table, torch.tensor([20], **I32),
+            torch.tensor([0, 1], **I32), torch.empty(1, 256, dtype=torch.bfloat16, device=DEV))
+    with pytest.raises(RuntimeError):
+        ops.attn_tree(*args, **kw)
+    ws.ws = whole
+    ops.attn_tree(*args, **kw)
