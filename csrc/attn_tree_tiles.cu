@@ -34,8 +34,8 @@
 //
 // Bound: the softmax threads' own time, 2100 cycles for a step of 64 tokens and 700
 // for its waits, while the products take about 800 and the loads less.  8 trees of 64
-// nodes x 4 heads over 8192 keys, 8 kv heads of 128, 8-bit cache: 160 us, 425 TFLOP/s
-// (134 MB).  With one row tile the loading warps, 3000 cycles for 128 tokens of the
+// nodes x 4 heads over 8192 keys, 8 kv heads of 128, 8-bit cache: 162 us, 420 TFLOP/s
+// (146 MB).  With one row tile the loading warps, 3000 cycles for 128 tokens of the
 // 8-bit cache: 64 sequences of 2048 keys, 20 rows, 143 us (bf16 cache 126 us, 4.3 TB/s).
 #include "attn_tree.cuh"
 #include "common.cuh"

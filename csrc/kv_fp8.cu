@@ -79,6 +79,8 @@ __device__ __forceinline__ uint2 pack8_e4m3(const float (&v)[8], float inv) {
 // A thread handles HPT heads of its token, all loaded before the first is used
 // (and before the cosines arrive); with few tokens the heads of a token spread
 // over gridDim.y CTAs instead.
+// Bound: memory.  8192 tokens of 32 + 2 x 8 heads of 128: 189 MB in 35 us, 5.5 TB/s.
+// A few tokens: two dependent trips to memory, 2 us behind another kernel.
 template <int D, int HPT>
 __global__ void __launch_bounds__(128) rope_kv_write_fp8_kernel(const WriteArgs a) {
   constexpr int LPH = D / 16;
@@ -198,6 +200,8 @@ struct ReadArgs {
 // A thread turns pieces of 8 codes into 8 bf16 values each: 8-byte loads and
 // 16-byte stores, both whole lines for a warp, and kReadPieces of them in
 // flight.  Pieces run over [block][K, V][head][token][dim].
+// Bound: memory, two thirds of it writes.  4096 blocks of 8 heads of 128: 407 MB in
+// 80 us, 5.1 TB/s.
 constexpr int kReadPieces = 8;
 
 template <int D>

@@ -175,3 +175,31 @@ def test_refusals():
               (x, t, -1), (x[:, :4], t, 5), (x, t.cpu(), 1), (x.cpu(), t, 1)):
         with pytest.raises((RuntimeError, ValueError)):
             ops.token_logprobs(*a)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("k", [0, 1, 20])
+def test_many_rows(dtype, k):
+    g = torch.Generator().manual_seed(k)
+    x = (torch.randn(1301, 5003, generator=g) * 3).to(dtype)
+    t = torch.randint(0, 5003, (1301,), generator=g).to(torch.int32)
+    _check(x.to(DEV), t.to(DEV), k)
+
+
+@pytest.mark.parametrize("rows", [1, 700])
+@pytest.mark.parametrize("k", [2, 32])
+def test_largest_values_all_in_a_few_places(rows, k):
+    """More values over the bound than fit: all of one thread in 32's, and (one row)
+    all of a few slices'."""
+    g = torch.Generator().manual_seed(k + rows)
+    x = torch.randn(rows, 131072, generator=g).to(torch.bfloat16)
+    chunk = torch.arange(131072) // 8
+    x[:, chunk % 32 == 5] += 40.0
+    t = torch.randint(0, 131072, (rows,), generator=g).to(torch.int32)
+    _check(x.to(DEV), t.to(DEV), k)
+    if rows == 1:
+        v = 1200000
+        slices = ops.ext().token_logprobs_plan(1, v, 4)[0]
+        x = torch.randn(1, v, generator=g)
+        x[:, torch.arange(v) // (-(-v // slices)) % 32 == 3] -= 60.0
+        _check(x.to(DEV), t.to(DEV), k)
