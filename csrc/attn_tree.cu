@@ -18,8 +18,8 @@
 // own for every row: exact down to 2^-9 of the row's largest value, and to 2^-18 of
 // it below that.  The codes of V are exact in fp16, and the weights are held in fp16
 // too, times a power of two (11 bits down to 2^-27, the rest of them to within 2^-37),
-// and summed as 2^8 w / vs, which stays finite for 2^19 keys down to the smallest
-// scale, 2^-100.  (Weights as sums of 8-bit numbers would spare V's unpacking.  Two
+// and summed as 2^6 w / vs, which stays finite for 2^19 keys (w up to 4, see kLag)
+// down to the smallest scale, 2^-100.  (Weights as sums of 8-bit numbers would spare V's unpacking.  Two
 // e4m3 parts lose all below 2^-18 of the largest: the many small weights beside one
 // large one.  Four e5m2 parts hold them, but double the products of V: 150 us against
 // 132 when tried.)  With the bf16 cache the weights are rounded to bf16, as
@@ -71,8 +71,8 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], u
 
 constexpr float kLag = 2.f;   // scores may pass the maximum in use by a factor 2^kLag
 constexpr float kUp = 13.f;   // fp16 weights are held as 2^kUp w: at most 2^(kUp + kLag)
-constexpr float kSum = 8.f;   // and summed as 2^kSum w / vs
-constexpr float kBack = 1.f / 32;  // 2^(kSum - kUp)
+constexpr float kSum = 6.f;   // and summed as 2^kSum w / vs
+constexpr float kBack = 1.f / 128;  // 2^(kSum - kUp)
 
 __device__ __forceinline__ float lg2(float x) {
   float y;
