@@ -602,8 +602,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tiles_kernel(const Args 
         for (int j = 0; j < steps; ++j, ++n) {
           const int kc = kc0 + (two ? j / kSpt : w + j / kSpt * 2), sg = kc & 1;
           const int buf = n % kSb, part = j % kSpt;
-          if (part == 0 && !warp_wait(v_full + sg, (kc >> 1) & 1, a.status, abort_flag)) break;
+          // Weights first: they come only after the job before has been finished by both
+          // groups, all its tiles of values read.  Until then the values' barrier may be
+          // two phases behind this tile's, which a wait on its parity takes for done: with
+          // one row tile this group does not wait for the other one's tiles.
           if (!warp_wait(p_bar + buf, (n / kSb) & 1, a.status, abort_flag)) break;
+          if (part == 0 && !warp_wait(v_full + sg, (kc >> 1) & 1, a.status, abort_flag)) break;
           tc_fence_after();
           const uint64_t vd =
               v_desc + (uint32_t)(sg * (S::kVTile >> 4) + part * (kStep * 128 >> 4));

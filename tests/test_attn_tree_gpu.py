@@ -400,3 +400,38 @@ def test_refuses_a_misaligned_workspace():
         ops.attn_tree(*args, **kw)
     ws.ws = whole
     ops.attn_tree(*args, **kw)
+
+
+@pytest.mark.parametrize("cache", ["fp8", "bf16"])
+@pytest.mark.parametrize("hq,hkv,d,nodes", [(8, 2, 128, 5), (4, 1, 64, 17), (12, 4, 128, 40)])
+def test_many_short_jobs_of_odd_tile_counts(cache, hq, hkv, d, nodes):
+    """More jobs of one row tile than SMs, of one to three K / V tiles (and some without
+    keys): a CTA goes from job to job with the tiles' stages left at either one, and a
+    softmax group without a tile of its own at times."""
+    g = torch.Generator().manual_seed(nodes)
+    lens = [int(torch.randint(128 * t + 1, 128 * t + 129, (1,), generator=g))
+            for t in torch.randint(0, 3, (420,), generator=g).tolist()]
+    rows = [min(n, nodes) for n in lens]
+    lens[::13] = [0] * len(lens[::13])
+    rows[::13] = [1] * len(rows[::13])
+    p = Problem(cache, hq, hkv, d, lens, rows, seed=nodes)
+    a = p.run(max_nodes=64)
+    p.check(a)
+    for _ in range(20):
+        assert torch.equal(p.run(max_nodes=64), a)
+    assert ops.read_status(torch.device(DEV)) == 0
+
+
+@pytest.mark.parametrize("cache", ["fp8", "bf16"])
+def test_jobs_of_one_and_two_row_tiles_in_turn(cache):
+    """Jobs whose K / V tiles the softmax groups take in turn beside jobs whose tiles
+    they share."""
+    g = torch.Generator().manual_seed(77)
+    lens = torch.randint(64, 520, (330,), generator=g).tolist()
+    rows = [(7, 64, 20, 64, 33)[i % 5] for i in range(330)]
+    p = Problem(cache, 8, 2, 128, lens, rows, seed=78)
+    a = p.run(max_nodes=64)
+    p.check(a)
+    for _ in range(20):
+        assert torch.equal(p.run(max_nodes=64), a)
+    assert ops.read_status(torch.device(DEV)) == 0
