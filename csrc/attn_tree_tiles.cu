@@ -538,6 +538,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tiles_kernel(const Args 
   const int64_t u0 = (int64_t)blockIdx.x * piece;
   const int64_t u_end = min(total, u0 + piece);
   volatile int* abort_flag = &s_abort;
+  // The softmax groups and the warps that issue the scores leave every job together.
+  // (A score warp without a tile in a job would not be missed otherwise: two jobs on,
+  // the query rows' barrier shows it the parity it had before, and it waits for ever.)
+  auto job_end = [] { named_bar_sync(3, 256 + 64); };
 
   if (warp >= 16) {
     // -------------------------------------------------------------- products
@@ -563,10 +567,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tiles_kernel(const Args 
       const Segment g = segment_at(a, pre, u, u_end, piece, *abort_flag != 0);
       u += g.units;
       const int nt = same(g.nt), two = same(g.mt == 2 ? 1 : 0);
-      if (nt == 0) continue;
-      const int steps = same(kSpt * group_tiles(nt, two + 1, w));
+      int steps = same(kSpt * group_tiles(nt, two + 1, w));
       if (!is_sum) {
-        if (!warp_wait(q_full, seg++ & 1, a.status, abort_flag)) continue;
+        if (nt > 0 && !warp_wait(q_full, seg++ & 1, a.status, abort_flag)) steps = 0;
         const uint64_t qd = q_desc + (uint32_t)((w & two) * (S::kQTile >> 4));
         for (int j = 0; j < steps; ++j, ++n) {
           const int kc = kc0 + (two ? j / kSpt : w + j / kSpt * 2), sg = kc & 1;
@@ -598,6 +601,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tiles_kernel(const Args 
           }
           __syncwarp();
         }
+        job_end();
       } else {
         for (int j = 0; j < steps; ++j, ++n) {
           const int kc = kc0 + (two ? j / kSpt : w + j / kSpt * 2), sg = kc & 1;
@@ -1029,7 +1033,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tiles_kernel(const Args 
       // The next job's query rows and statistics take the same places: not
       // before both groups are done with these.
       tc_fence_before();
-      named_bar_sync(2, 256);
+      job_end();
     }
   }
   tc_fence_before();

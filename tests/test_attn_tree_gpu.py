@@ -435,3 +435,23 @@ def test_jobs_of_one_and_two_row_tiles_in_turn(cache):
     for _ in range(20):
         assert torch.equal(p.run(max_nodes=64), a)
     assert ops.read_status(torch.device(DEV)) == 0
+
+
+@pytest.mark.parametrize("cache", ["fp8", "bf16"])
+@pytest.mark.parametrize("last", [0, 300])
+def test_a_softmax_group_without_tiles_keeps_up(cache, last):
+    """Job after job of a single K / V tile, all of them one group's, and none at all;
+    then one that needs both groups."""
+    g = torch.Generator().manual_seed(last)
+    lens = torch.randint(5, 129, (900,), generator=g).tolist()
+    lens[::9] = [0] * len(lens[::9])
+    rows = [5 if n else 1 for n in lens]
+    if last:
+        lens += [last] * 7
+        rows += [40] * 7
+    p = Problem(cache, 16, 4, 64, lens, rows, seed=11)
+    a = p.run(max_nodes=64)
+    p.check(a)
+    for _ in range(10):
+        assert torch.equal(p.run(max_nodes=64), a)
+    assert ops.read_status(torch.device(DEV)) == 0
