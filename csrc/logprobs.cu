@@ -6,10 +6,12 @@
 //
 // hold for every reference r near the row's maximum: each thread keeps its own
 // (r, S, W) and moves r only when a value is 2^8 times over it, so the common
-// path is one fused multiply-add and one exponential a value (the same r stands
-// in every term, so its own rounding cancels).  Above 1e29 in magnitude two
-// different floats are so far apart that S is the number of values equal to
-// the maximum.
+// path is one fused multiply-add and one exponential a value.  The same r stands
+// in every term, so its own rounding cancels, as long as 2^(that rounding) is a
+// finite number: below 2^30 r is rounded by 2^5 at most, so S stays below 2^72.
+// If the row's maximum is 2^29 or more in magnitude, other floats are so far from it
+// (32 at least) that S is the number of values equal to it.  Values of -2^30 or
+// less beside a maximum above -2^29 weigh nothing in any frame, and set none.
 //
 // Top k: each thread notes the chunk of its own largest value.  Of the largest
 // values of 32 groups of threads the k-th is a bound below the row's k-th largest,
@@ -166,8 +168,8 @@ __device__ __forceinline__ void block_rank(const Key* cand, int count, int k, Ke
 struct Stat {
   float m, r, s, w;
 };
-constexpr float kLowest = -1e30f;  // r of a thread without a finite value
-constexpr float kHuge = 1e29f;
+constexpr float kLowest = -1073741824.f;  // -2^30: r of a thread without a larger value
+constexpr float kHuge = 536870912.f;      // 2^29
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -221,13 +223,13 @@ template <typename T>
 struct Chunk {
   static constexpr int N = 16 / sizeof(T);
   float v[N];
-  // The largest of them, a NaN if there is one; with the values no lower than -1e30
+  // The largest of them, a NaN if there is one; with the values no lower than -2^30
   // from here on if that comes cheap (`bounded`).
   static constexpr bool bounded = std::is_same<T, __nv_bfloat16>::value;
   __device__ __forceinline__ float set_top(uint4 u) {
     if constexpr (bounded) {
       const uint32_t t = max_nan_bf16x2(max_nan_bf16x2(u.x, u.y), max_nan_bf16x2(u.z, u.w));
-      constexpr uint32_t kLow = 0xf14af14au;  // -1e30, twice
+      constexpr uint32_t kLow = 0xce80ce80u;  // -2^30, twice
       u.x = max_bf16x2(u.x, kLow);
       u.y = max_bf16x2(u.y, kLow);
       u.z = max_bf16x2(u.z, kLow);
@@ -325,7 +327,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) token_logprobs_kernel(const Ar
   if (edge >= 0) {
     edge_v = value(x + edge);
     nan |= edge_v != edge_v;
-    if (edge_v > kLowest && edge_v < kHuge) raise(edge_v);
+    if (edge_v * kLog2e > st.r && edge_v < kHuge) raise(edge_v);
     add(edge_v, false);
   }
   int c = tid;

@@ -203,3 +203,44 @@ def test_largest_values_all_in_a_few_places(rows, k):
         x = torch.randn(1, v, generator=g)
         x[:, torch.arange(v) // (-(-v // slices)) % 32 == 3] -= 60.0
         _check(x.to(DEV), t.to(DEV), k)
+
+
+@pytest.mark.parametrize("rows", [1, 700])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("mask", [-1e8, -1e9, -1e10, -1e12, -1e20, -1e28, -1e29, -7e29, -1e30,
+                                  -1e35])
+def test_large_finite_masks(rows, dtype, mask):
+    """Whole runs of a row at a large negative number, as masks leave them: their
+    probability is 0, and the others are as without them."""
+    g = torch.Generator().manual_seed(rows)
+    x = (torch.randn(rows, 20001, generator=g) * 5).to(dtype)
+    x[:, :12000] = mask             # most threads see nothing else
+    x[torch.rand(rows, 20001, generator=g) < 0.3] = mask
+    x[:, 20000] = mask
+    if rows > 1:
+        x[1] = mask                 # every token alike
+        x[2] = mask
+        x[2, 777] = -3.0            # one token left
+    t = torch.randint(0, 20001, (rows,), generator=g).to(torch.int32)
+    _check(x.to(DEV), t.to(DEV), 9)
+
+
+@pytest.mark.parametrize("rows", [1, 700])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("top", [1e7, 1e8, 4e8, 6e8, 1e9, 2e9, 1e10, 1e20, 1e28, 2e29])
+def test_rows_of_large_logits(rows, dtype, top):
+    """Maxima of either sign far from 0, alone, in a few equal values, and with
+    neighbours at the distance of the type's numbers there."""
+    g = torch.Generator().manual_seed(int(top) % 1000)
+    x = torch.randn(rows, 9003, generator=g) * 3
+    x = torch.where(torch.rand(rows, 9003, generator=g) < 0.5, -top * (1.5 + x.abs()), x)
+    x[0] = -top * (1 + torch.rand(9003, generator=g))
+    x[0, [5, 4000, 9002]] = -top
+    if rows > 1:
+        x[1, [17, 5000]] = top
+        x[2] = top * (1 - torch.rand(9003, generator=g) * 1e-6)
+        x[3] = -top * (1 + torch.rand(9003, generator=g) * 1e-6)
+    x = x.to(dtype)
+    t = torch.randint(0, 9003, (rows,), generator=g).to(torch.int32)
+    t[0] = 4000
+    _check(x.to(DEV), t.to(DEV), 6)
