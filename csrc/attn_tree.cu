@@ -803,13 +803,18 @@ void attn_tree(at::Tensor q, at::Tensor k_cache, at::Tensor v_cache,
                   row_start.numel() >= B + 1,
               "int32 block tables [B, W], seq lens [B] and row starts [B + 1]");
   for (const at::Tensor* t :
-       {&out, &k_cache, &v_cache, &block_tables, &seq_lens, &row_start, &ws, &counters})
+       {&out, &k_cache, &v_cache, &block_tables, &seq_lens, &row_start, &ws, &counters, &status})
     TORCH_CHECK(t->device() == q.device(), "all tensors must be on one device");
+  auto aligned16 = [](const at::Tensor& t) {
+    return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  };
+  TORCH_CHECK(aligned16(k_cache) && aligned16(v_cache), "k/v cache must be 16-byte aligned");
   if (fp8) {
     for (const at::Tensor* t : {&*k_scale, &*v_scale})
       TORCH_CHECK(t->scalar_type() == at::kFloat && t->is_contiguous() &&
                       t->numel() == k_cache.numel() / D && t->device() == q.device(),
                   "k/v scales must be fp32 [L, NB, Hkv, 16] contiguous");
+    TORCH_CHECK(aligned16(*k_scale) && aligned16(*v_scale), "k/v scales must be 16-byte aligned");
   }
   if (masks.has_value())
     TORCH_CHECK(masks->scalar_type() == at::kLong && masks->is_contiguous() &&
@@ -817,14 +822,14 @@ void attn_tree(at::Tensor q, at::Tensor k_cache, at::Tensor v_cache,
                 "masks must be int64, one per row");
   TORCH_CHECK(max_nodes >= 1 && (!masks.has_value() || max_nodes <= 64),
               "a tree has at most 64 nodes");
-  TORCH_CHECK((q.stride(0) * 2) % 16 == 0 && reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0,
+  TORCH_CHECK((q.stride(0) * 2) % 16 == 0 && aligned16(q),
               "q rows must be 16-byte aligned");
   if (B == 0 || q.size(0) == 0) return;
   const c10::cuda::CUDAGuard guard(q.device());
   const std::vector<int64_t> plan = attn_tree_plan(D);
   TORCH_CHECK(ws.scalar_type() == at::kFloat && ws.numel() >= plan[1] &&
                   counters.scalar_type() == at::kInt && counters.numel() >= plan[2] &&
-                  reinterpret_cast<uintptr_t>(ws.data_ptr()) % 16 == 0,
+                  aligned16(ws) && status.scalar_type() == at::kInt && status.numel() >= 1,
               "workspace too small, or not 16-byte aligned");
   tree::Args a;
   a.q = reinterpret_cast<const __nv_bfloat16*>(q.data_ptr());

@@ -258,6 +258,9 @@ static void check_fp8_cache(const at::Tensor& k, const at::Tensor& v,
   TORCH_CHECK(k.dim() == 5 && k.size(3) == 16 && k.is_contiguous() && v.is_contiguous() &&
                   v.sizes() == k.sizes(),
               "k/v cache must be [L, NB, Hkv, 16, D] contiguous, of one shape");
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(k.data_ptr()) % 8 == 0 &&
+                  reinterpret_cast<uintptr_t>(v.data_ptr()) % 8 == 0,
+              "k/v cache must be 8-byte aligned");
   TORCH_CHECK(ks.scalar_type() == at::kFloat && vs.scalar_type() == at::kFloat && ks.dim() == 4 &&
                   ks.is_contiguous() && vs.is_contiguous() && ks.sizes() == vs.sizes() &&
                   ks.size(0) == k.size(0) && ks.size(1) == k.size(1) && ks.size(2) == k.size(2) &&

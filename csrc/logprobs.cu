@@ -556,8 +556,9 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> token_logprobs(
   const std::vector<int64_t> plan = token_logprobs_plan(R, V, es);
   TORCH_CHECK(ws.scalar_type() == at::kFloat && counters.scalar_type() == at::kInt &&
                   ws.device() == logits.device() && counters.device() == logits.device() &&
-                  ws.numel() >= plan[1] && counters.numel() >= plan[2],
-              "workspace too small");
+                  ws.numel() >= plan[1] && counters.numel() >= plan[2] &&
+                  (plan[0] == 1 || reinterpret_cast<uintptr_t>(ws.data_ptr()) % 16 == 0),
+              "workspace too small, or not 16-byte aligned");
   lp::Args a;
   a.x = logits.data_ptr();
   a.ld = logits.stride(0);
