@@ -10,7 +10,8 @@
 // in every term, so its own rounding cancels, as long as 2^(that rounding) is a
 // finite number: below 2^30 r is rounded by 2^5 at most, so S stays below 2^72.
 // If the row's maximum is 2^29 or more in magnitude, other floats are so far from it
-// (32 at least) that S is the number of values equal to it.  Values of -2^30 or
+// (32 at least) that S is the number of values equal to it.  At the end r moves to the
+// maximum itself, the thread's and then the row's.  Values of -2^30 or
 // less beside a maximum above -2^29 weigh nothing in any frame, and set none.
 //
 // Top k: each thread notes the chunk of its own largest value.  Of the largest
@@ -301,12 +302,12 @@ __global__ void __launch_bounds__(kThreads, CTAS) token_logprobs_kernel(const Ar
     st.s *= f;
     st.r = r;
   };
-  auto add = [&](float v, bool bounded) {
+  auto add = [&](float v, bool bounded, float& s, float& w) {
     float d = fmaf(v, kLog2e, -st.r);
     if (!bounded) d = fmaxf(d, -200.f);  // -inf: a weight of 0, not a NaN
     const float e = ex2(d);
-    st.s += e;
-    st.w = fmaf(e, d, st.w);
+    s += e;
+    w = fmaf(e, d, w);
   };
   auto take = [&](const uint4& raw, int c) {
     Chunk<T> u;
@@ -317,8 +318,13 @@ __global__ void __launch_bounds__(kThreads, CTAS) token_logprobs_kernel(const Ar
       best = c;
     }
     if (top * kLog2e > st.r + 8.f && top < kHuge) raise(top);
+    // A chunk's sums on their own first: W counts the lag of r, up to 8 S, and every sum
+    // with it is rounded by that much.
+    float s = 0.f, w = 0.f;
 #pragma unroll
-    for (int i = 0; i < N; ++i) add(u.v[i], Chunk<T>::bounded);
+    for (int i = 0; i < N; ++i) add(u.v[i], Chunk<T>::bounded, s, w);
+    st.s += s;
+    st.w += w;
   };
   // Edges: fewer than 2 N elements, one for each of the first threads.
   const int n0 = v0 - lo;
@@ -328,7 +334,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) token_logprobs_kernel(const Ar
     edge_v = value(x + edge);
     nan |= edge_v != edge_v;
     if (edge_v * kLog2e > st.r && edge_v < kHuge) raise(edge_v);
-    add(edge_v, false);
+    add(edge_v, false, st.s, st.w);
   }
   int c = tid;
   for (; c + (U - 1) * kThreads < chunks; c += U * kThreads) {
@@ -348,6 +354,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) token_logprobs_kernel(const Ar
       if (c + i * kThreads < chunks) take(raw[i], c + i * kThreads);
   }
   st.m = nan ? __int_as_float(0x7fc00000) : fmaxf(best_v, edge_v);
+  if (st.m * kLog2e > st.r && st.m < kHuge) raise(st.m);  // no lag from here on
 
   // This thread's largest value with its index.
   Key key = 0;
@@ -488,19 +495,25 @@ __global__ void __launch_bounds__(kThreads, CTAS) token_logprobs_kernel(const Ar
     st = stats[0];
   }
   if (warp != 0) return;
+  // From the rounded reference to the maximum: S counts the maximum itself as 1 and is
+  // no less, so that no probability passes 1 and no entropy falls below 0.
+  if (!bad && !empty && !far) {
+    const float d = fmaf(m, kLog2e, -st.r), f = ex2(-d);
+    st.w = f * fmaf(-st.s, d, st.w);
+    st.s *= f;
+  }
   constexpr float kLn2 = 0.6931471805599453f;
-  const float log2_s = log2f(st.s);
+  const float log2_s = log2f(fmaxf(st.s, 1.f));
   const float none = __int_as_float(0x7fc00000);
   auto lp_of = [&](float v) {
     if (bad) return none;
-    if (empty || v == -INFINITY) return -INFINITY;
-    if (far || fabsf(v) >= kHuge) return (v - m) - log2_s * kLn2;  // v log2e may overflow
-    return (fmaf(v, kLog2e, -st.r) - log2_s) * kLn2;
+    if (empty) return -INFINITY;
+    return fmaf(-log2_s, kLn2, v - m);
   };
   if (lane == 0) {
     const int t = a.tokens[row];
     a.logprob[row] = t >= 0 && t < a.V ? lp_of(value(x + t)) : none;
-    a.entropy[row] = bad ? none : (empty ? 0.f : (log2_s - st.w / st.s) * kLn2);
+    a.entropy[row] = bad ? none : (empty ? 0.f : fmaxf(log2_s - st.w / st.s, 0.f) * kLn2);
   }
   if (lane < a.top_k) {
     a.top_ids[(int64_t)row * a.top_k + lane] = (int)~(uint32_t)top;

@@ -244,3 +244,33 @@ def test_rows_of_large_logits(rows, dtype, top):
     t = torch.randint(0, 9003, (rows,), generator=g).to(torch.int32)
     t[0] = 4000
     _check(x.to(DEV), t.to(DEV), 6)
+
+
+@pytest.mark.parametrize("rows", [1, 64, 700])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_confident_rows(rows, dtype):
+    """One token far over the rest, after values that rise in small steps: a probability
+    is at most 1, an entropy at least 0."""
+    g = torch.Generator().manual_seed(rows)
+    x = torch.randn(rows, 30011, generator=g) * 0.3
+    top = torch.rand(rows, generator=g) * 40 + 12
+    at = torch.randint(0, 30011, (rows,), generator=g)
+    # The way up to the maximum, in the places before it that its thread reads.
+    for back in range(1, 5):
+        i = at - back * 512 * (4 if dtype == torch.float32 else 8)
+        x[torch.arange(rows)[i >= 0], i[i >= 0]] = (top - 5 * back)[i >= 0]
+    x[torch.arange(rows), at] = top
+    x = x.to(dtype)
+    lp, ent, _, best = _check(x.to(DEV), at.to(torch.int32).to(DEV), 3)
+    assert bool((lp <= 0).all()) and bool((best <= 0).all()) and bool((ent >= 0).all())
+
+
+@pytest.mark.parametrize("gap", [3.0, 5.0, 8.0, 20.0, 60.0])
+def test_certain_token(gap):
+    """A token that has all but e^-gap of the probability; rows in many frames."""
+    x = torch.zeros(257, 40) - gap
+    x[:, 7] = 0.0
+    x += torch.linspace(-30, 30, 257)[:, None]
+    t = torch.full((257,), 7, dtype=torch.int32)
+    lp, ent, _, best = _check(x.to(DEV), t.to(DEV), 2)
+    assert bool((lp <= 0).all()) and bool((best <= 0).all()) and bool((ent >= 0).all())
