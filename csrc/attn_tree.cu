@@ -736,12 +736,8 @@ __global__ void __launch_bounds__(128, rows_ctas<D, FP8, NR>()) attn_rows_kernel
 template <int D, bool FP8, int NR>
 void launch_rows(const Args& a, cudaStream_t stream) {
   const int smem = Smem<D, FP8, NR>::bytes(a.B);
-  static int configured = 0;
-  if (smem > configured) {
-    CB_CUDA_CHECK(cudaFuncSetAttribute(attn_rows_kernel<D, FP8, NR>,
-                                       cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    configured = smem;
-  }
+  static PerDevice allowed;
+  allow_smem(attn_rows_kernel<D, FP8, NR>, Smem<D, FP8, NR>::bytes(kMaxBatch), allowed);
   // A whole number of CTAs for each kv head.
   const int per_head = std::max(1, rows_ctas<D, FP8, NR>() * num_sms() / a.Hkv);
   launch_kernel(attn_rows_kernel<D, FP8, NR>, dim3(per_head * a.Hkv), dim3(128), smem, stream, a);

@@ -1045,16 +1045,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tiles_kernel(const Args 
 template <int D, bool FP8>
 void launch_tiles(const Args& a, cudaStream_t stream) {
   const int smem = TileSmem<D, FP8>::bytes(a.B);
-  static int configured = 0;
-  if (smem > configured) {
-    CB_CUDA_CHECK(cudaFuncSetAttribute(attn_tiles_kernel<D, FP8>,
-                                       cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  static PerDevice allowed, checked;
+  allow_smem(attn_tiles_kernel<D, FP8>, TileSmem<D, FP8>::bytes(kMaxBatch), allowed);
+  checked.once(0, [] {
     cudaFuncAttributes attr;
     CB_CUDA_CHECK(cudaFuncGetAttributes(&attr, attn_tiles_kernel<D, FP8>));
     if (attr.numRegs < kRegsLaunch)  // the groups' shares would never come free
       throw std::runtime_error("attn_tiles_kernel was built with too few registers a thread");
-    configured = smem;
-  }
+  });
   launch_kernel(attn_tiles_kernel<D, FP8>, dim3(num_sms()), dim3(kTileThreads), smem, stream, a);
 }
 

@@ -12,6 +12,8 @@
 #include <string>
 #include <utility>
 
+#include "per_device.h"
+
 #define CB_CUDA_CHECK(expr)                                                              \
   do {                                                                                   \
     cudaError_t _e = (expr);                                                             \
@@ -69,6 +71,18 @@ inline void launch_kernel(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_
   cfg.attrs = attr;
   cfg.numAttrs = pdl_flag() ? 1 : 0;
   CB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...));
+}
+
+// Lets a kernel have `bytes` of dynamic shared memory on the current device: the most
+// that any of its launches asks for, so that no launch lowers what another has set.
+template <typename... KArgs>
+inline void allow_smem(void (*kernel)(KArgs...), int bytes, PerDevice& set) {
+  int device = 0;
+  CB_CUDA_CHECK(cudaGetDevice(&device));
+  set.once(device, [&] {
+    CB_CUDA_CHECK(
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  });
 }
 
 using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
