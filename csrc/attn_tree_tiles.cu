@@ -24,7 +24,10 @@
 // rounded up, so that a softmax thread needs one number a tile for them instead of
 // two for each column (shared-memory bandwidth).  The price is one rounding to
 // fp16's 11 bits, 2^-12 of a value against the 2^-5 of its code and the 2^-9 of the
-// bf16 result; the scale itself enters as a pair of fp16 numbers, 22 bits.
+// bf16 result; the scale itself enters as a pair of fp16 numbers, 22 bits.  Scales far
+// below the reference would lose bits, and all of them beside a hidden or weightless
+// key with a large one: a tile whose scales span 2^kSpan or more takes an r for each key,
+// at the cost of the slower pass over its scores.
 //
 // Weights are computed in one pass over the scores, in the frame of the maximum
 // that the row had before; only if a score is more than 2^8 over it (or keys of
@@ -57,6 +60,8 @@ static_assert(2 * kRegsSoftmax + 2 * kRegsLoad + kRegsIssue <= 5 * kRegsLaunch,
 static_assert(kRegsLoad <= kRegsLaunch && kRegsIssue <= kRegsLaunch && kRegsLaunch <= kRegsSoftmax,
               "a share may only shrink below the launch's, or grow above it");
 constexpr int kTileBufs = 8;       // tiles whose scale references are kept
+constexpr int kSpan = 12;          // log2 of the span of scales that share one
+constexpr float kEachItsOwn = 1e9f;  // in place of a tile's reference
 
 template <int D, bool FP8>
 struct TileSmem {
@@ -70,7 +75,8 @@ struct TileSmem {
   static constexpr int kRaw = kQ + 2 * kQTile;       // V's codes as they come: [2][128][D]
   static constexpr int kScale = kRaw + (FP8 ? 2 * 128 * D : 0);  // K's: [kTileBufs][128] fp32
   static constexpr int kPairs = kScale + kTileBufs * kTok * 4;  // V's: [8 warps][128]
-  static constexpr int kMl = kPairs + 8 * kTok * 4;  // [2][128][2]
+  static constexpr int kRefs = kPairs + 8 * kTok * 4;  // keys' own references: [kTileBufs][128]
+  static constexpr int kMl = kRefs + (FP8 ? kTileBufs * kTok * 4 : 0);  // [2][128][2]
   static constexpr int kBars = kMl + 2 * 128 * 2 * 4;
   static constexpr int kPre = kBars + 256;
   static int bytes(int B) { return kPre + (B + 2) / 2 * 2 * 8 + 1024; }
@@ -275,7 +281,8 @@ struct LoadSmem {
   uint32_t raw;       // this lane's place in V's codes
   uint32_t pairs;     // this warp's [128] scales of V over the reference, as fp16 pairs
   float* k_scale;     // [kTileBufs][128]
-  float* v_ref;       // [kTileBufs]: log2 of V's reference / 2^6
+  float* v_ref;       // [kTileBufs]: log2 of V's reference / 2^6, or kEachItsOwn
+  float* v_refs;      // [kTileBufs][128]: the same for each key
   uint64_t *k_full, *v_full, *k_free, *v_free;  // [2]
   uint64_t* r_full;   // [kTileBufs]
   volatile int* abort_flag;
@@ -376,7 +383,7 @@ __device__ __forceinline__ void load_tiles(const Args& a, const int64_t* pre, in
       const bool tail = pos0 + kTok > g.ctx;
       if constexpr (FP8) {
         float kx[4] = {ks.x, ks.y, ks.z, ks.w}, vx[4] = {vs.x, vs.y, vs.z, vs.w};
-        uint32_t top = 0u;
+        uint32_t top = 0u, low = 0xffffffffu;  // of the scales that are not 0
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           // A row past the end gets the scale 0.  A key one of whose scales is not
@@ -386,17 +393,21 @@ __device__ __forceinline__ void load_tiles(const Args& a, const int64_t* pre, in
           if (!fine) kx[e] = __int_as_float(0x7fc00000);
           if (!fine || (tail && pos0 + 4 * lane + e >= g.len)) vx[e] = 0.f;
           top = max(top, __float_as_uint(vx[e]));
+          if (vx[e] != 0.f) low = min(low, __float_as_uint(vx[e]));
         }
         // Reference 2^(x - 126) > the tile's largest scale.  x is kept from 43 on
         // (2^-83; 127 without any scale): sums of weights over the reference stay
         // far from overflow then, even for heads whose values are all zero.
         top = __reduce_max_sync(0xffffffffu, top);
         const int x = top == 0u ? 127 : max(43, (int)(top >> 23));
-        const float factor = __int_as_float((253 - x) << 23) * 64.f;  // 2^6 / reference
+        low = __reduce_min_sync(0xffffffffu, low);
+        const bool wide = top != 0u && x - max(43, (int)(low >> 23)) >= kSpan;
         uint32_t pair[4];  // each token's scale over the reference as two fp16 numbers
+        int own[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float y = vx[e] * factor;
+          own[e] = wide && vx[e] != 0.f ? max(43, (int)(__float_as_uint(vx[e]) >> 23)) : x;
+          const float y = vx[e] * (__int_as_float((253 - own[e]) << 23) * 64.f);  // 2^6 s / r
           pair[e] = pack_f16(y, y - __half2float(__float2half_rn(y)));
         }
         __syncwarp();
@@ -406,7 +417,10 @@ __device__ __forceinline__ void load_tiles(const Args& a, const int64_t* pre, in
           const int slot = kc & (kTileBufs - 1);
           reinterpret_cast<float4*>(sm.k_scale + slot * kTok)[lane] =
               make_float4(kx[0], kx[1], kx[2], kx[3]);
-          if (lane == 0) sm.v_ref[slot] = (float)(x - 126 - 6);
+          reinterpret_cast<float4*>(sm.v_refs + slot * kTok)[lane] =
+                make_float4((float)(own[0] - 126 - 6), (float)(own[1] - 126 - 6),
+                            (float)(own[2] - 126 - 6), (float)(own[3] - 126 - 6));
+          if (lane == 0) sm.v_ref[slot] = wide ? kEachItsOwn : (float)(x - 126 - 6);
           mbar_arrive(sm.r_full + slot);
         }
         if (more) {
@@ -474,6 +488,85 @@ __device__ __forceinline__ void load_tiles(const Args& a, const int64_t* pre, in
   copies_wait<0>();
 }
 
+// A step of a softmax thread's row in two passes over its scores, the maximum first:
+// where keys are hidden, where the row's maximum moves, and for values with a
+// reference each.  (A call, so that its registers stay out of the ordinary step's: with
+// the keys' references in line the trees of 64 nodes took 185 to 215 us.)
+struct StepEnd {
+  float m, l;
+  bool ok;
+};
+
+template <int D, bool FP8>
+__device__ __noinline__ StepEnd two_pass_step(uint32_t s_addr, uint32_t o_addr, const float* sc,
+                                              const float* refs, float mul, float m, float l,
+                                              RowSight sight, int pos0, bool tail, bool has_sums,
+                                              uint64_t* pv_bar, uint32_t pv_parity, int* status,
+                                              volatile int* abort_flag) {
+  constexpr float kUp = FP8 ? 7.f : 0.f;
+  bool ok = true;
+  float mx = -INFINITY;
+#pragma unroll 1
+  for (int c0 = 0; c0 < kStep; c0 += 32) {
+    uint32_t v[32];
+    __syncwarp();
+    tmem_ld32_start(s_addr + c0, v);
+    tmem_ld32_wait(v);
+    const uint32_t seen = tail ? sight.at(pos0 + c0) : 0xffffffffu;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const float x = __uint_as_float(v[i]);
+      const float t = FP8 ? fmaf(x * sc[c0 + i], mul, refs[c0 + i]) : x * mul;
+      mx = fmaxf(mx, seen >> i & 1 ? t : -INFINITY);
+    }
+  }
+  float alpha = 1.f;
+  if (mx > m) {
+    alpha = ex2(m - mx);
+    m = mx;
+    l *= alpha;
+  }
+  if (__any_sync(0xffffffffu, alpha != 1.f) && has_sums) {
+    ok = warp_wait(pv_bar, pv_parity, status, abort_flag);
+    tc_fence_after();
+#pragma unroll 1
+    for (int c0 = 0; c0 < D; c0 += 16) {
+      float v[16];
+      __syncwarp();
+      tmem_ld16(o_addr + c0, v);
+      uint32_t w[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(v[i] * alpha);
+      tmem_st16(o_addr + c0, w);
+    }
+  }
+  const float shift = kUp - m;
+#pragma unroll 1
+  for (int c0 = 0; c0 < kStep; c0 += 32) {
+    uint32_t v[32];
+    __syncwarp();
+    tmem_ld32_start(s_addr + c0, v);
+    tmem_ld32_wait(v);
+    const uint32_t seen = tail ? sight.at(pos0 + c0) : 0xffffffffu;
+    uint32_t w[16];
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) {
+      float t[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float x = __uint_as_float(v[i + e]), r = FP8 ? refs[c0 + i + e] : 0.f;
+        t[e] = ex2(FP8 ? fmaf(x * sc[c0 + i + e], mul, r + shift) : fmaf(x, mul, shift));
+        if (!(seen >> (i + e) & 1)) t[e] = 0.f;
+        // (the weights count the values' reference: 2^r of it out again)
+        l = FP8 ? fmaf(t[e], ex2(-r), l) : l + t[e];
+      }
+      w[i / 2] = FP8 ? pack_f16(t[0], t[1]) : pack_bf16(t[0], t[1]);
+    }
+    tmem_st16(s_addr + c0 / 2, w);
+  }
+  return {m, l, ok};
+}
+
 template <int D, bool FP8>
 __global__ void __launch_bounds__(kTileThreads, 1) attn_tiles_kernel(const Args a) {
   using S = TileSmem<D, FP8>;
@@ -483,6 +576,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tiles_kernel(const Args 
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
   float* k_scale = reinterpret_cast<float*>(smem + S::kScale);
+  float* v_refs = reinterpret_cast<float*>(smem + S::kRefs);
   float* sm_ml = reinterpret_cast<float*>(smem + S::kMl);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kBars);
   uint64_t* k_full = bars;        // [2]
@@ -642,6 +736,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tiles_kernel(const Args 
     sm.pairs = smem_u32(smem + S::kPairs) + (warp - 8) * kTok * 4;
     sm.k_scale = k_scale;
     sm.v_ref = s_vref;
+    sm.v_refs = v_refs;
     sm.k_full = k_full;
     sm.v_full = v_full;
     sm.k_free = k_free;
@@ -763,7 +858,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tiles_kernel(const Args 
           const float lv = FP8 ? s_vref[kc & (kTileBufs - 1)] : 0.f;
           const float* sc = k_scale + (kc & (kTileBufs - 1)) * kTok + j % kSpt * kStep;
           const bool tail = pos0 + kStep > g.ctx;
-          bool again = __any_sync(0xffffffffu, tail || m == kNegBig);
+          const bool wide = FP8 && lv == kEachItsOwn;
+          const float* refs = v_refs + (kc & (kTileBufs - 1)) * kTok + j % kSpt * kStep;
+          bool again = __any_sync(0xffffffffu, tail || wide || m == kNegBig);
           float sum = 0.f;
           if (!again) {
             const F2 mul2v = f2(mul, mul);
@@ -816,69 +913,16 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tiles_kernel(const Args 
             }
           }
           if (again) {
-            // Two passes: the step's maximum first.
-            auto scaled = [&](uint32_t acc, int c) {
-              return FP8 ? __uint_as_float(acc) * sc[c] : __uint_as_float(acc);
-            };
-            float mx = -INFINITY;
-#pragma unroll 1
-            for (int c0 = 0; c0 < kStep; c0 += 32) {
-              uint32_t v[32];
-              __syncwarp();
-              tmem_ld32_start(s_addr + c0, v);
-              tmem_ld32_wait(v);
-              const uint32_t seen = tail ? sight.at(pos0 + c0) : 0xffffffffu;
-#pragma unroll
-              for (int i = 0; i < 32; ++i)
-                mx = fmaxf(mx, seen >> i & 1 ? fmaf(scaled(v[i], c0 + i), mul, lv) : -INFINITY);
-            }
-            float alpha = 1.f;
-            if (mx > m) {
-              alpha = ex2(m - mx);
-              m = mx;
-              l *= alpha;
-            }
-            if (__any_sync(0xffffffffu, alpha != 1.f) && j > 0) {
-              ok = warp_wait(pv_done + 2 * wg + (n - 1) % kSb, ((n - 1) / kSb) & 1, a.status,
-                             abort_flag);
-              tc_fence_after();
-#pragma unroll 1
-              for (int c0 = 0; c0 < D; c0 += 16) {
-                float v[16];
-                __syncwarp();
-                tmem_ld16(o_addr + c0, v);
-                uint32_t w[16];
-#pragma unroll
-                for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(v[i] * alpha);
-                tmem_st16(o_addr + c0, w);
-              }
-            }
-            const float shift = lv + kUp - m;
-            sum = 0.f;
-#pragma unroll 1
-            for (int c0 = 0; c0 < kStep; c0 += 32) {
-              uint32_t v[32];
-              __syncwarp();
-              tmem_ld32_start(s_addr + c0, v);
-              tmem_ld32_wait(v);
-              const uint32_t seen = tail ? sight.at(pos0 + c0) : 0xffffffffu;
-              uint32_t w[16];
-#pragma unroll
-              for (int i = 0; i < 32; i += 2) {
-                float t[2];
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                  t[e] = ex2(fmaf(scaled(v[i + e], c0 + i + e), mul, shift));
-                  if (!(seen >> (i + e) & 1)) t[e] = 0.f;
-                  sum += t[e];
-                }
-                w[i / 2] = FP8 ? pack_f16(t[0], t[1]) : pack_bf16(t[0], t[1]);
-              }
-              tmem_st16(s_addr + c0 / 2, w);
-            }
+            const StepEnd e = two_pass_step<D, FP8>(
+                s_addr, o_addr, sc, refs, mul, m, l, sight, pos0, tail, j > 0,
+                pv_done + 2 * wg + (n - 1) % kSb, ((n - 1) / kSb) & 1, a.status, abort_flag);
+            m = e.m;
+            l = e.l;
+            ok = e.ok;
+          } else {
+            // (the weights count the values' reference: 2^lv of it out again)
+            l += FP8 ? sum * ex2(-lv) : sum;
           }
-          // (the weights count the values' reference: 2^lv of it out again)
-          l += FP8 ? sum * ex2(-lv) : sum;
           tmem_st_wait();
         }
         if (!ok) break;

@@ -455,3 +455,42 @@ def test_a_softmax_group_without_tiles_keeps_up(cache, last):
     for _ in range(10):
         assert torch.equal(p.run(max_nodes=64), a)
     assert ops.read_status(torch.device(DEV)) == 0
+
+
+@pytest.mark.parametrize("cache", ["fp8", "bf16"])
+@pytest.mark.parametrize("nodes", [1, 5, 40])
+@pytest.mark.parametrize("far", [2.0 ** 14, 2.0 ** 25, 2.0 ** 40, 2.0 ** 100])
+def test_a_large_value_that_does_not_count(cache, nodes, far):
+    """Beside the others' values a key's is far larger, but hidden (a node that only
+    itself sees) or of no weight (a score far below the others): the others keep
+    their bits."""
+    ctx = 150
+    for hidden in (True, False):
+        if hidden and nodes == 1:
+            continue
+        at = ctx + 1 if hidden else 70
+        p = Problem(cache, 8, 2, 128, [ctx + nodes, 31], [nodes, 1], seed=21,
+                    v_mul=lambda shape, g: torch.where(
+                        (torch.arange(shape[0]) == at).view(-1, 1, 1), far, 1.0))
+        if hidden:
+            p.masks[:nodes] = [1 << i | 1 for i in range(nodes)]
+        else:
+            # Every query has 8 in its first place, this key alone something against it.
+            low = -140.0 - 12 * math.log2(far) * (far > 2.0 ** 40)
+            p = Problem(cache, 8, 2, 128, [ctx + nodes, 31], [nodes, 1], seed=21,
+                        v_mul=lambda shape, g: torch.where(
+                            (torch.arange(shape[0]) == at).view(-1, 1, 1), far, 1.0))
+            p.q.view(-1, 8, 128)[:, :, 0] = 8.0
+            blk, row = int(p.table[0, at // 16]), at % 16
+            x = torch.zeros(2, 128)
+            x[:, 0] = low
+            if cache == "fp8":
+                codes, s = ref.quantise_rows(x)
+                p.kc.view(torch.uint8)[p.layer, blk, :, row] = codes.view(torch.uint8).to(DEV)
+                p.ks[p.layer, blk, :, row] = s.to(DEV)
+                p.kf[p.layer, blk, :, row] = ref.dequantise_rows(codes, s)
+            else:
+                p.kc[p.layer, blk, :, row] = x.to(torch.bfloat16).to(DEV)
+                p.kf[p.layer, blk, :, row] = x.to(torch.bfloat16).float()
+        p.check(p.run())
+        p.check(p.run(max_nodes=64))
