@@ -366,7 +366,7 @@ class LLMEngine(Engine):
     def _spec_decode_trees(self, seqs: List[Sequence], out):
         """One speculative round with n-gram trees; sequences that asked for
         logprobs take part (the verification computes them)."""
-        from ..runtime.spec import MAX_TREE_NODES, NGramDraft, verify_trees
+        from ..runtime.spec import MAX_TREE_NODES, NGramDraft, fit_trees, verify_trees
 
         m = self.model
         trees = []
@@ -378,9 +378,10 @@ class LLMEngine(Engine):
                        self.max_model_len - s.total_len - 1) - 1
             trees.append(s.ngram.propose_tree(self.spec_k, min(31, MAX_TREE_NODES)).cut(
                 max(0, room)))
+        ids, lens = [s.seq_id for s in seqs], [s.total_len - 1 for s in seqs]
+        trees = fit_trees(m.kv, ids, lens, trees)
         k = max(min(20, s.task.logprobs) for s in seqs)
-        results = verify_trees(m, [s.seq_id for s in seqs], [s.output_ids[-1] for s in seqs],
-                               trees, [s.total_len - 1 for s in seqs], k)
+        results = verify_trees(m, ids, [s.output_ids[-1] for s in seqs], trees, lens, k)
         if self._device_failed(seqs, out):
             return
         st = self.spec_stats

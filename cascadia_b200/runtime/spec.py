@@ -174,6 +174,10 @@ class DraftTree:
                 keep[i + 1] = new.add(keep[p], t)
         return new
 
+    def first(self, n: int) -> "DraftTree":
+        """The first ``n`` drafted nodes (parents come before their children)."""
+        return DraftTree(self.tokens[:n], self.parents[:n])
+
 
 def count_accepted(drafts: Sequence[int], target: Sequence[int]) -> int:
     """Length of the longest prefix where the draft equals the target's pick."""
@@ -402,6 +406,23 @@ class TreeResult:
     draft_logprob: float         # mean log-probability the target gave first drafts
 
 
+def fit_trees(kv, seq_ids: Sequence[str], kv_lens: Sequence[int],
+              trees: Sequence[DraftTree]) -> List[DraftTree]:
+    """The trees with as many nodes as the pool has slots for, beside the one
+    that every sequence's pending token takes: a round of trees never needs a
+    block that plain decoding would not have to have."""
+    have = [max(len(kv.seqs[s].blocks), -(-(p0 + 1) // BLOCK_SIZE))
+            for s, p0 in zip(seq_ids, kv_lens)]
+    spare = max(0, kv.allocator.num_free - sum(h - len(kv.seqs[s].blocks)
+                                               for s, h in zip(seq_ids, have)))
+    out = []
+    for p0, blocks, tree in zip(kv_lens, have, trees):
+        more = min(spare, max(0, -(-(p0 + 1 + len(tree.tokens)) // BLOCK_SIZE) - blocks))
+        spare -= more
+        out.append(tree.first((blocks + more) * BLOCK_SIZE - p0 - 1))
+    return out
+
+
 def build_tree_batch(m, seq_ids: Sequence[str], trees: Sequence[DraftTree],
                      kv_lens: Sequence[int]):
     """The inputs of one forward over every sequence's pending token and
@@ -411,9 +432,15 @@ def build_tree_batch(m, seq_ids: Sequence[str], trees: Sequence[DraftTree],
 
     kv, dev = m.kv, m.device
     pos, slots, ctx, masks, counts = [], [], [], [], []
+    try:
+        for sid, tree, p0 in zip(seq_ids, trees, kv_lens):
+            kv.reserve(sid, p0 + 1 + len(tree.tokens))
+    except MemoryError:
+        for sid, p0 in zip(seq_ids, kv_lens):
+            kv.truncate(sid, p0)
+        raise
     for sid, tree, p0 in zip(seq_ids, trees, kv_lens):
         n = 1 + len(tree.tokens)
-        kv.reserve(sid, p0 + n)
         st = kv.seqs[sid]
         st.length = max(st.length, p0 + n)
         pos.extend(p0 + d for d in tree.depths())
@@ -827,6 +854,7 @@ class TreeSpecDecoder:
             # Never draft past the token budget.
             trees = [t.cut(max(0, max_new_tokens - s.generated - 1))
                      for (_, s), t in zip(live, trees)]
+            trees = fit_trees(m.kv, [s.sid for _, s in live], [s.kv_len for _, s in live], trees)
             t1 = time.perf_counter()
             results = verify_trees(m, [s.sid for _, s in live], [s.tokens[-1] for _, s in live],
                                    trees, [s.kv_len for _, s in live])

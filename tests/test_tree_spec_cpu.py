@@ -244,3 +244,74 @@ def test_builder_and_moe_family_take_the_8_bit_cache():
     e.submit(GenerationTask("a", "", max_tokens=8, prompt_ids=[5, 6, 7, 5, 6, 7, 5, 6]))
     out = _drain(e, ["a"])["a"]
     assert len([c for c in out if not c.is_final]) in range(1, 9)
+
+
+# ------------------------------------------------------------ a tight pool
+def _tight(blocks, kv_dtype="bf16", seed=5):
+    m = LlamaModel(get_config("tiny-llama"), "cpu").init_random(seed=seed, gen_device="cpu")
+    m.allocate_kv(blocks, kv_dtype=kv_dtype)
+    return m
+
+
+@pytest.mark.parametrize("draft", ["ngram", "self"])
+def test_trees_in_a_pool_that_plain_decoding_just_fits(draft):
+    new = 20
+    blocks = sum(-(-(len(p) + new - 1) // 16) for p in _prompts())
+    want = BatchGenerator(_tight(blocks), use_graph=False).generate(_prompts(), new)
+    with pytest.raises(MemoryError):
+        BatchGenerator(_tight(blocks - 1), use_graph=False).generate(_prompts(), new)
+    m = _tight(blocks)
+    dm = None if draft == "ngram" else _model(seed=5)
+    dec = TreeSpecDecoder(m, draft=dm, k=4, branch=4, max_nodes=40, use_graph=False)
+    assert dec.generate(_prompts(), new) == want
+    assert m.kv.allocator.num_free == blocks
+    if draft == "self":  # there is still room for some drafts
+        assert dec.stats.accepted > 0
+
+
+def test_engine_trees_in_a_pool_that_plain_decoding_just_fits():
+    new = 20
+    got = {}
+    blocks = sum(-(-(len(p) + new) // 16) for p in _prompts())
+    for spec in (None, "tree"):
+        e = LLMEngine(_tight(blocks), max_model_len=48, spec=spec, spec_k=6, use_graph=False)
+        for i, p in enumerate(_prompts()):
+            e.submit(GenerationTask(f"t{i}", "", max_tokens=new, prompt_ids=p))
+        if spec:
+            # Drafts of many branches for every sequence, wrong ones.
+            from cascadia_b200.runtime import spec as spec_mod
+
+            old = spec_mod.NGramDraft.propose_tree
+            spec_mod.NGramDraft.propose_tree = lambda self, k, most: DraftTree.from_chains(
+                [[3 + i, 4 + i, 5 + i] for i in range(9)], most)
+        try:
+            out = _drain(e, ["t0", "t1", "t2"])
+        finally:
+            if spec:
+                spec_mod.NGramDraft.propose_tree = old
+        got[spec] = [[c.token_id for c in out[f"t{i}"] if not c.is_final] for i in range(3)]
+        assert e.model.kv.allocator.num_free == blocks
+    assert got["tree"] == got[None] and all(len(x) >= 1 for x in got[None])
+
+
+def test_a_failed_reservation_gives_back_what_it_took():
+    m = _tight(6)
+    g = BatchGenerator(m, use_graph=False)
+    prompts = [list(range(3, 18)), list(range(3, 34)), [5]]
+    g.prefill(["a", "b", "c"], prompts)
+    lens = [len(p) for p in prompts]
+    before = {s: list(m.kv.seqs[s].blocks) for s in "abc"}
+    wide = DraftTree()
+    for i in range(40):
+        wide.add(0, i)
+    with pytest.raises(MemoryError):
+        verify_trees(m, ["a", "b", "c"], [4, 4, 4], [DraftTree(), wide, DraftTree()], lens)
+    assert {s: m.kv.seqs[s].blocks for s in "abc"} == before
+    assert [m.kv.seqs[s].length for s in "abc"] == lens
+    # What fits is drafted, in the order of the nodes.
+    from cascadia_b200.runtime.spec import fit_trees
+
+    cut = fit_trees(m.kv, ["a", "b", "c"], lens, [wide, wide, wide])
+    assert [len(t.tokens) for t in cut] == [32, 0, 14]
+    assert cut[0].tokens == wide.tokens[:32]
+    verify_trees(m, ["a", "b", "c"], [4, 4, 4], cut, lens)
