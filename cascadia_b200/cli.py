@@ -157,6 +157,10 @@ def validate_run_flags(args) -> None:
         bad("--spec draft needs --draft-model")
     if args.spec == "tree" and getattr(args, "tp", 1) > 1:
         bad("--spec tree runs on one GPU")
+    if args.spec == "tree" and args.engine in ("mock", "dsv4", "moe"):
+        bad(f"--spec tree is served by --engine llama, not by --engine {args.engine}")
+    if getattr(args, "kv_dtype", "bf16") != "bf16" and args.engine in ("mock", "dsv4"):
+        bad(f"--engine {args.engine} has no --kv-dtype {args.kv_dtype}")
     if getattr(args, "kv_dtype", "bf16") != "bf16" and (pp > 1 or getattr(args, "ep", 1) > 1):
         bad("--kv-dtype fp8 is served without pipeline stages and expert parallelism")
     if tp > 1 and not os.path.isdir(str(args.model)):
@@ -332,6 +336,10 @@ def cmd_worker(args):
     _init_logging(args.log_level)
     if args.rank >= args.total:
         raise SystemExit(f"--rank {args.rank} must be < --total {args.total}")
+    if args.kv_dtype != "bf16":
+        raise SystemExit("--kv-dtype fp8 is served without pipeline stages (run)")
+    if args.spec == "tree":
+        raise SystemExit("--spec tree is served without pipeline stages (run)")
     name = args.served_model_name or os.path.basename(str(args.model).rstrip("/"))
     nl = _num_layers(args.model)
     if args.layer_start is not None and args.layer_end is not None:

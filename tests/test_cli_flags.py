@@ -56,3 +56,29 @@ def test_good_combinations_pass():
     cli.validate_run_flags(_args(model="llama-3.1-8b", tp=8))
     cli.validate_run_flags(_args(tp=2, pp=2))
     cli.validate_run_flags(_args(spec="draft", draft_model="tiny-llama"))
+
+
+@pytest.mark.parametrize("kw, msg", [
+    (dict(engine="mock", kv_dtype="fp8"), "--kv-dtype"),
+    (dict(engine="dsv4", kv_dtype="fp8"), "--kv-dtype"),
+    (dict(engine="mock", spec="tree"), "--spec tree"),
+    (dict(engine="dsv4", spec="tree"), "--spec tree"),
+    (dict(engine="moe", model="tiny-moe", spec="tree"), "--spec tree"),
+])
+def test_engines_without_the_8_bit_cache_or_trees_refuse_them(kw, msg):
+    with pytest.raises(SystemExit) as e:
+        cli.validate_run_flags(_args(**kw))
+    assert msg in str(e.value)
+
+
+def test_engines_with_the_8_bit_cache_and_trees():
+    cli.validate_run_flags(_args(kv_dtype="fp8", spec="tree"))
+    cli.validate_run_flags(_args(engine="moe", model="tiny-moe", kv_dtype="fp8"))
+    cli.validate_run_flags(_args(engine="mock", kv_dtype="bf16"))
+
+
+@pytest.mark.parametrize("flags", [["--kv-dtype", "fp8"], ["--spec", "tree"]])
+def test_a_pipeline_worker_refuses_them(flags):
+    with pytest.raises(SystemExit) as e:
+        cli.main(["worker", "--rank", "0", "--total", "1", "--device", "cpu"] + flags)
+    assert flags[0] in str(e.value)
