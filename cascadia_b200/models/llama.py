@@ -432,9 +432,12 @@ class LlamaModel:
             q = qkv[:, :hq * d]
             win, sinks = self.cfg.sliding_window, self.cfg.attention_sinks
             if batch.masks is not None or (kv.fp8 and batch.is_decode):
-                ops.attn_tree(q, kv.k, kv.v, batch.block_tables, batch.seq_lens,
-                              batch.rows_of_seqs(), out, li, self.scale, masks=batch.masks,
-                              k_scale=kv.k_scale, v_scale=kv.v_scale, max_nodes=batch.max_nodes)
+                starts, most = batch.rows_of_seqs(), ops.ATTN_TREE_MAX_SEQS
+                for b in range(0, batch.seq_lens.numel(), most):
+                    ops.attn_tree(q, kv.k, kv.v, batch.block_tables[b:b + most],
+                                  batch.seq_lens[b:b + most], starts[b:b + most + 1], out, li,
+                                  self.scale, masks=batch.masks, k_scale=kv.k_scale,
+                                  v_scale=kv.v_scale, max_nodes=batch.max_nodes)
             elif batch.is_decode:
                 ops.attn_decode(q, kv.k, kv.v, batch.block_tables, batch.seq_lens, out, li,
                                 batch.num_splits, batch.blocks_per_split, batch.part_o,

@@ -283,6 +283,9 @@ def decode_split_plan(batch: int, kv_heads: int, max_blocks: int, num_sms: int =
     return splits, bps
 
 
+ATTN_TREE_MAX_SEQS = 2048  # sequences of one attn_tree call
+
+
 @functools.lru_cache(maxsize=16)
 def _attn_tree_plan(head_dim: int) -> tuple:
     return tuple(ext().attn_tree_plan(head_dim)[1:])
@@ -302,7 +305,7 @@ def attn_tree(q, k_cache, v_cache, block_tables, seq_lens, row_start, out, layer
     entry (int64 [rows]) is set; without masks the keys j <= i.  A row that
     sees nothing gives zeros.  Lengths are read on the device, so a captured
     graph follows them.  ``max_nodes``: an upper bound on the rows of a
-    sequence (at most 64 with masks)."""
+    sequence (at most 64 with masks).  At most ATTN_TREE_MAX_SEQS sequences."""
     if _dbg.ENABLED and not torch.cuda.is_current_stream_capturing():
         _dbg.check_paged(block_tables, seq_lens, k_cache.shape[1])
         _dbg.check_range("rows", row_start[1:] - row_start[:-1], 0, max_nodes + 1)

@@ -156,3 +156,22 @@ def test_engine_logprobs(kv_dtype, spec):
         assert len(c.logprobs.top_logprobs) == 5
         assert c.logprobs.top_logprobs[0].logprob >= c.logprobs.top_logprobs[4].logprob
         assert abs(c.logprobs.top_logprobs[0].logprob - float(top[0, 0])) < 0.1
+
+
+def test_more_sequences_than_one_attention_call_takes():
+    """Decoding and chain verification of thousands of rows on the 8-bit cache."""
+    g = torch.Generator().manual_seed(8)
+    few = torch.randint(3, 500, (60, 5), generator=g).tolist()
+    prompts = [few[i % 60] for i in range(2100)]
+    m = LlamaModel(get_config("tiny-llama"), "cuda").init_random(seed=5, gen_device="cpu")
+    m.allocate_kv(2100, kv_dtype="fp8")
+    want = BatchGenerator(m).generate(few, 6)
+    got = BatchGenerator(m).generate(prompts, 6)
+    same = sum(_agree(a, want[i % 60]) for i, a in enumerate(got))
+    assert same >= 0.8 * 6 * 2100
+    # 600 sequences of 5 rows each in a captured verification.
+    draft = LlamaModel(get_config("tiny-llama"), "cuda").init_random(seed=5, gen_device="cpu")
+    draft.allocate_kv(1200)
+    got = SpecDecoder(m, draft=draft, k=4).generate(few * 10, 6)
+    assert sum(_agree(a, want[i % 60]) for i, a in enumerate(got)) >= 0.7 * 6 * 600
+    assert ops.read_status(torch.device("cuda")) == 0
