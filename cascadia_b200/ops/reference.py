@@ -139,6 +139,23 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: flo
     return torch.where(total == 0, torch.zeros_like(o), o / total)
 
 
+def top_ids(x: torch.Tensor, k: int) -> torch.Tensor:
+    """Indices [R, k] of the largest values of rows, larger first, then lower
+    index; a NaN comes before every number."""
+    k = min(k, x.shape[1])
+    if k == 0:
+        return torch.zeros(x.shape[0], 0, dtype=torch.long, device=x.device)
+    least = x.topk(k, dim=-1).values[:, -1:]
+    out = torch.empty(x.shape[0], k, dtype=torch.long, device=x.device)
+    for row, reach, ids in zip(x, x >= least, out):
+        # (a NaN reaches nothing, and nothing reaches a NaN: such rows are sorted whole)
+        at = reach.nonzero()[:, 0]
+        if len(at) < k or bool(row.amax().isnan()):
+            at = torch.arange(len(row), device=x.device)
+        ids.copy_(at[torch.sort(row[at], descending=True, stable=True).indices[:k]])
+    return out
+
+
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0):
     """(logprob, entropy, ids, top) of logit rows; see ops.token_logprobs."""
     x = logits if logits.dtype == torch.float64 else logits.float()
@@ -148,17 +165,24 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0):
     sh = x - torch.where(empty, torch.zeros_like(m), m)
     e = torch.exp(sh)
     S = e.sum(-1, keepdim=True)
-    lp = torch.where(bad, torch.full_like(x, float("nan")),
-                     torch.where(empty, torch.full_like(x, float("-inf")), sh - S.log()))
-    ent = -torch.where(e > 0, e * lp, torch.zeros_like(x)).sum(-1) / S[:, 0]
+    log_s = S.log()
+
+    def lp_of(at):
+        lp = sh.gather(1, at) - log_s
+        lp = torch.where(empty, torch.full_like(lp, float("-inf")), lp)
+        return torch.where(bad, torch.full_like(lp, float("nan")), lp)
+
+    # (0 log 0 = 0: a value of -inf takes no part in the sum of e sh)
+    spread = (e * sh.clamp_min(torch.finfo(x.dtype).min)).sum(-1) / S[:, 0]
+    ent = log_s[:, 0] - spread
     ent = torch.where(bad[:, 0], torch.full_like(ent, float("nan")),
                       torch.where(empty[:, 0], torch.zeros_like(ent), ent))
-    ids = torch.sort(x, dim=-1, descending=True, stable=True).indices[:, :top_k]
+    ids = top_ids(x, top_k)
     t = tokens.long()
     known = (t >= 0) & (t < x.shape[1])
-    got = lp.gather(1, t.clamp(0, x.shape[1] - 1).unsqueeze(1))[:, 0]
+    got = lp_of(t.clamp(0, x.shape[1] - 1).unsqueeze(1))[:, 0]
     got = torch.where(known, got, torch.full_like(got, float("nan")))
-    return got, ent, ids.to(torch.int32), lp.gather(1, ids)
+    return got, ent, ids.to(torch.int32), lp_of(ids)
 
 
 def argmax(logits: torch.Tensor) -> torch.Tensor:
