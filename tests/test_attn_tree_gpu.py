@@ -494,3 +494,79 @@ def test_a_large_value_that_does_not_count(cache, nodes, far):
                 p.kf[p.layer, blk, :, row] = x.to(torch.bfloat16).float()
         p.check(p.run())
         p.check(p.run(max_nodes=64))
+
+
+def test_tile_kernel_past_32_bits():
+    """Rows at the far end of a pool of more than 2^32 codes, read by the tile kernel."""
+    hkv, d, n = 8, 128, 300
+    nb = (1 << 32) // (hkv * 16 * d) + 40
+    p = Problem("fp8", 16, hkv, d, [n, 70], [40, 64], seed=17, layers=1, layer=0, spare=0)
+    want = p.run()
+    p.check(want)
+    pools = []
+    used = p.kc.shape[1]
+    for small in (p.kc, p.vc):
+        big = torch.empty(1, nb, hkv, 16, d, dtype=torch.uint8, device=DEV)
+        big[:, nb - used:] = small.view(torch.uint8)
+        pools.append(big.view(torch.float8_e4m3fn))
+    for small in (p.ks, p.vs):
+        big = torch.empty(1, nb, hkv, 16, device=DEV)
+        big[:, nb - used:] = small
+        pools.append(big)
+    p.kc, p.vc, p.ks, p.vs = pools
+    p.table = p.table + (nb - used)
+    assert torch.equal(p.run(max_nodes=64), want)
+
+
+def test_tile_kernel_past_32_bits_with_an_infinite_node():
+    """The same for the bf16 cache, whose infinities are read a second time."""
+    hkv, d, n = 8, 128, 150
+    nb = (1 << 32) // (hkv * 16 * d) + 40
+    p = Problem("bf16", 16, hkv, d, [n], [40], seed=19, layers=1, layer=0, spare=0)
+    blk = int(p.table[0, (n - 37) // 16])  # node 3
+    p.vc[0, blk, :, (n - 37) % 16, 5] = float("inf")
+    want = p.run()
+    sees = torch.tensor([bool(m >> 3 & 1) for m in p.masks])
+    got = want.view(40, 16, d)
+    assert bool((got[sees][:, :, 5] == float("inf")).all()) and bool(got[~sees].isfinite().all())
+    used = p.kc.shape[1]
+    pools = []
+    for small in (p.kc, p.vc):
+        big = torch.empty(1, nb, hkv, 16, d, dtype=torch.bfloat16, device=DEV)
+        big[:, nb - used:] = small
+        pools.append(big)
+    p.kc, p.vc = pools
+    p.table = p.table + (nb - used)
+    assert torch.equal(p.run(max_nodes=64), want)
+
+
+@pytest.mark.parametrize("cache", ["fp8", "bf16"])
+@pytest.mark.parametrize("nodes", [1, 5, 40])
+@pytest.mark.parametrize("c,a", [(2.0 ** -9, 1.0), (2.0 ** -9, 0.25), (2.0 ** -9, -0.296875),
+                                 (2.0 ** -6, 2.0 ** -5)])
+def test_products_are_summed_in_32_bits(cache, nodes, c, a):
+    """Two keys that differ by 127 small products beside a product of 448 to 448 000
+    times their size: sums of fewer bits would lose them."""
+    p = Problem(cache, 4, 1, 128, [2 + nodes], [nodes], seed=23)
+    p.masks = [0] * nodes
+    p.scale = 1.0
+    p.q = torch.full((nodes, 4, 128), a)
+    p.q[:, :, 0] = 1.0
+    p.q = p.q.view(nodes, 512).to(torch.bfloat16)
+    k = torch.zeros(2, 1, 128)
+    k[0] = c
+    k[:, :, 0] = 448.0
+    v = torch.zeros(2, 1, 128)
+    v[0] = 1.0
+    blk = int(p.table[0, 0])
+    for x, pool, full, scale in ((k, p.kc, p.kf, p.ks), (v, p.vc, p.vf, p.vs)):
+        for t in range(2):
+            if cache == "fp8":
+                codes = x[t].to(torch.float8_e4m3fn)
+                assert torch.equal(codes.float(), x[t])
+                pool.view(torch.uint8)[p.layer, blk, :, t] = codes.view(torch.uint8).to(DEV)
+                scale[p.layer, blk, :, t] = 1.0
+            else:
+                pool[p.layer, blk, :, t] = x[t].to(torch.bfloat16).to(DEV)
+            full[p.layer, blk, :, t] = x[t]
+    p.check(p.run())
