@@ -2,12 +2,17 @@
 
     python bench/bench_tree_spec.py [--model llama-3.1-8b] [--batch 8] [--prompt-len 2048]
                                     [--new 128] [--kv-dtype fp8] [--draft ngram|exit|none]
+                                    [--follow-text 0]
 
-Every prompt repeats a short passage, so n-gram drafts find something to
-propose; ``exit`` drafts with the target's own first layers (early exit).
-Weights are random (INT4, seeded).  Prints one JSON line: tokens per second of
-plain decoding and of tree decoding, accepted drafts per round, and the mean
-log-probability of the emitted tokens.
+Every prompt repeats a short passage.  Weights are random (INT4, seeded), but for the
+embedding's size and the LM head's rows of the passages' tokens, which are set so that the
+model goes on with the passage: n-gram drafts are right then, and so are those of ``exit``
+(the target's own first layers), as the best case of speculation.  ``--follow-text 0``
+leaves the weights as they are: nothing predicts what the model emits, n-gram drafts find
+nothing to propose and the others are not accepted, the cost of speculation where it does
+not help.  Prints one JSON line: tokens per second of plain decoding and of tree decoding,
+nodes drafted and tokens emitted per round, and the mean log-probability of the emitted
+tokens.
 """
 import argparse
 import json
@@ -21,9 +26,21 @@ import torch  # noqa: E402
 
 from cascadia_b200 import ops  # noqa: E402
 from cascadia_b200.models.config import get_config  # noqa: E402
-from cascadia_b200.models.llama import LlamaModel  # noqa: E402
+from cascadia_b200.models.llama import Int4Weight, LlamaModel, QLinear  # noqa: E402
 from cascadia_b200.runtime.generator import BatchGenerator  # noqa: E402
 from cascadia_b200.runtime.spec import TreeSpecDecoder  # noqa: E402
+
+
+def follow_text(m, passages):
+    """Make the token after each of a passage's the model's own choice: the residual is
+    mostly the embedding, and the head's row of the next token points along it."""
+    head = torch.randn(m.cfg.vocab_size, m.cfg.hidden_size, device=m.device,
+                       generator=torch.Generator(m.device).manual_seed(2)) * 0.02
+    for text in passages:
+        at = torch.tensor(text, device=m.device)
+        head[at.roll(-1)] = m.embed[at].float() / m.embed.float().std() * 0.1
+    m.embed.mul_(100.0 / m.embed.float().std())
+    m.lm_head = QLinear(Int4Weight.quantize(head, m.cfg.group_size), m.device)
 
 
 def main():
@@ -38,18 +55,20 @@ def main():
     p.add_argument("--k", type=int, default=6, help="depth of a tree")
     p.add_argument("--branch", type=int, default=3)
     p.add_argument("--nodes", type=int, default=31)
+    p.add_argument("--follow-text", type=int, default=1)
     a = p.parse_args()
     dev = torch.device("cuda")
     m = LlamaModel(get_config(a.model), dev).init_random(seed=0)
     width = -(-(a.prompt_len + a.new + 80) // 16)
     m.allocate_kv(a.batch * width + 64, kv_dtype=a.kv_dtype)
     g = torch.Generator().manual_seed(1)
-    prompts = []
-    for _ in range(a.batch):
-        text = torch.randint(3, m.cfg.vocab_size, (61,), generator=g).tolist()
-        prompts.append((text * (a.prompt_len // 61 + 1))[:a.prompt_len])
+    passages = [torch.randint(3, m.cfg.vocab_size, (61,), generator=g).tolist()
+                for _ in range(a.batch)]
+    prompts = [(text * (a.prompt_len // 61 + 1))[:a.prompt_len] for text in passages]
+    if a.follow_text:
+        follow_text(m, passages)
     out = {"model": a.model, "batch": a.batch, "prompt_len": a.prompt_len, "new": a.new,
-           "kv_dtype": a.kv_dtype, "kv_bytes_per_token": m.kv_bytes_per_block(a.kv_dtype) // 16}
+           "follow_text": a.follow_text, "kv_dtype": a.kv_dtype, "kv_bytes_per_token": m.kv_bytes_per_block(a.kv_dtype) // 16}
 
     def timed(fn):
         fn(8)  # captures, caches
