@@ -745,8 +745,8 @@ void launch_rows(const Args& a, cudaStream_t stream) {
 
 // By the query rows of a kv head and sequence.  64 sequences of 2048 keys, 8 kv heads
 // of 128, 8-bit cache (bf16): 8 rows 59 us here and 78 with room for 16 (93 and 94); 16
-// rows 100 and 85 (169 and 101), 143 on the tile kernel (124); 20 rows 147 here, where
-// they read the keys twice, and 143 on the tile kernel (179 and 126).
+// rows 100 and 85 (169 and 101), 147 on the tile kernel (124); 20 rows 147 here, where
+// they read the keys twice, and 147 on the tile kernel (179 and 125), 48 rows 149 there.
 template <int D, bool FP8>
 void launch(const Args& a, int64_t max_rows, cudaStream_t stream) {
   if (max_rows <= 8)

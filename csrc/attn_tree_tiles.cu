@@ -37,9 +37,11 @@
 //
 // Bound: the softmax threads' own time, 2100 cycles for a step of 64 tokens and 700
 // for its waits, while the products take about 800 and the loads less.  8 trees of 64
-// nodes x 4 heads over 8192 keys, 8 kv heads of 128, 8-bit cache: 162 us, 420 TFLOP/s
-// (146 MB).  With one row tile the loading warps, 3000 cycles for 128 tokens of the
-// 8-bit cache: 64 sequences of 2048 keys, 20 rows, 143 us (bf16 cache 126 us, 4.3 TB/s).
+// nodes x 4 heads over 8192 keys, 8 kv heads of 128, 8-bit cache: 163 us, 418 TFLOP/s
+// (146 MB).  Some 50 us of it are not in the steps (56 for a CTA, 157 000 cycles): start,
+// ends of jobs and joins.  With one row tile the loading warps, 3000 cycles for 128 tokens
+// of the 8-bit cache: 64 sequences of 2048 keys, 20 rows, 147 us (bf16 cache 125 us,
+// 4.3 TB/s).
 #include "attn_tree.cuh"
 #include "common.cuh"
 #include "host_utils.h"

@@ -25,8 +25,8 @@
 // A row is cut in slices, one for each CTA, when there are few rows; the last
 // CTA of a row joins them.
 //
-// Bound: memory for many rows (2047 rows of 128256 bf16 logits, 525 MB: 97 us without
-// alternatives, 5.4 TB/s; 110 us with one), where the exponentials take about 60 us and
+// Bound: memory for many rows (2047 rows of 128256 bf16 logits, 525 MB: 98 us without
+// alternatives, 5.3 TB/s; 110 us with one), where the exponentials take about 60 us and
 // 16-bit logits' maxima are taken two at a time.  Latency for few: one row 9 us with
 // alternatives, 64 rows 16 us, for two trips to memory, two joins of a CTA and a launch.
 #include <ATen/core/Tensor.h>
