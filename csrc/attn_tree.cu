@@ -787,7 +787,8 @@ void attn_tree(at::Tensor q, at::Tensor k_cache, at::Tensor v_cache,
               "the 8-bit cache comes with k_scale and v_scale, the bf16 cache without");
   const int D = (int)k_cache.size(4), Hkv = (int)k_cache.size(2);
   TORCH_CHECK(D == 64 || D == 128, "head_dim must be 64 or 128");
-  TORCH_CHECK(q.size(1) % D == 0 && (q.size(1) / D) % Hkv == 0, "query heads must divide");
+  TORCH_CHECK(Hkv > 0 && q.size(1) > 0 && q.size(1) % D == 0 && (q.size(1) / D) % Hkv == 0,
+              "query heads must divide");
   TORCH_CHECK(Hkv <= 2 * num_sms(), "too many kv heads");
   TORCH_CHECK(layer >= 0 && layer < k_cache.size(0), "layer outside the cache");
   const int64_t B = seq_lens.numel();

@@ -297,7 +297,8 @@ void rope_kv_write_fp8(at::Tensor qkv, at::Tensor positions, at::Tensor cos_sin,
                   qkv.size(1) == (Hq + 2 * Hkv) * D,
               "qkv must be bf16 [T, (Hq + 2 Hkv) D] with inner stride 1");
   TORCH_CHECK(D == 64 || D == 128 || D == 256, "head_dim must be 64, 128 or 256");
-  TORCH_CHECK(k_cache.size(2) == Hkv && k_cache.size(4) == D, "cache heads / head_dim mismatch");
+  TORCH_CHECK(k_cache.size(2) == Hkv && k_cache.size(4) == D && Hq >= 0,
+              "cache heads / head_dim mismatch");
   TORCH_CHECK(rot > 0 && rot % 16 == 0 && rot <= D, "rotary dim must be a multiple of 16, <= D");
   TORCH_CHECK(layer >= 0 && layer < k_cache.size(0), "layer outside the cache");
   const int64_t T = qkv.size(0);
@@ -364,7 +365,7 @@ void kv_read_fp8(at::Tensor k_cache, at::Tensor v_cache, at::Tensor k_scale,
     TORCH_CHECK(o->device() == k_cache.device(), "all tensors must be on one device");
   }
   TORCH_CHECK(blocks.device() == k_cache.device(), "all tensors must be on one device");
-  if (N == 0) return;
+  if (N == 0 || Hkv == 0) return;
   const c10::cuda::CUDAGuard guard(k_cache.device());
   ReadArgs a;
   a.k = reinterpret_cast<const uint8_t*>(k_cache.data_ptr());
