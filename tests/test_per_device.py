@@ -17,7 +17,7 @@ PROGRAM = r"""
 #include <vector>
 #include "per_device.h"
 int main() {
-  // As a launch uses it: the limit of the current device, from a fake of the driver.
+  // As a launch uses it: the limit of the current device, from a fake of the CUDA runtime.
   static int limit[70];
   static std::atomic<int> calls[70];
   static cb::PerDevice set;
